@@ -176,6 +176,48 @@ int nb_g1_jacobian_ex(cudaStream_t stream, int nw, int nsub, const float* tape, 
 int nb_g1_diag_forward_ex(cudaStream_t stream, unsigned long long* counters, int nw, int nsub, int iterations,
                           const int* info, const float* tape, int tape_words);
 
+/* ---- training a policy through the step: layer norm, the global gradient norm and clipping -----------------------
+ * No counterpart in the reference (its gradients end at the step's inputs). Value types: 0 float32, 1 bfloat16,
+ * 2 float16. As every entry: asynchronous on `stream`, the caller owns every buffer, arguments out of range return
+ * cudaErrorInvalidValue before anything is launched, and results repeat bit for bit (no atomics).
+ *
+ * Layer norm of x (rows, cols), rows `stride` values apart (0: every row the same), y and g_x dense:
+ *   mean = sum x / cols, rstd = (sum (x - mean)^2 / cols + eps)^(-1/2), y = (x - mean) rstd weight + bias
+ * weight and bias (cols,) of type wtype, which is float32 or x's; each may be NULL (1 and 0). mean, rstd (rows,).
+ * The backward takes g_y (rows `g_stride` apart, x's type) and the forward's mean and rstd:
+ *   h = g_y weight, xh = (x - mean) rstd, g_x = rstd (h - mean(h) - xh mean(h xh)),
+ *   g_weight = sum over rows of g_y xh, g_bias = sum over rows of g_y (both of type wtype)
+ * g_x, g_weight and g_bias may each be NULL (not wanted); work: nb_g1_layer_norm_work_bytes(rows, cols) bytes, needed
+ * for g_weight or g_bias. With no rows g_weight and g_bias are zero. Sums are float32. */
+long long nb_g1_layer_norm_work_bytes(long long rows, long long cols);
+int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols, long long stride, int dtype,
+                             const void* x, int wtype, const void* weight, const void* bias, float eps, void* y,
+                             float* mean, float* rstd);
+int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long cols, long long g_stride,
+                              long long stride, int dtype, const void* g_y, const void* x, const float* mean,
+                              const float* rstd, int wtype, const void* weight, void* g_x, void* g_weight,
+                              void* g_bias, void* work);
+
+/* The list of `count` gradients, given by host arrays (read before the call returns): device addresses grads, value
+ * counts sizes (each tensor dense; 0 allowed), value types. S = the sum of all squares, in 64 bits; bad = the number
+ * of non-finite values. zero_nonfinite: those count as 0 in S and are written as 0; otherwise they take part as the
+ * arithmetic has them (S infinite or NaN).
+ *   sumsq: stats (2 doubles) = S, bad; ranks that share a model add theirs up before the next call.
+ *   scale: c = min(1, max_norm / (sqrt(S) + eps)), outs[i] = c grads[i] in type out_types[i]; norm = sqrt(S) and bad,
+ *     each where not NULL. An output may be its own gradient (same address and type); outputs that overlap anything
+ *     else are refused. outs NULL: norm and bad alone.
+ *   clip: sumsq, then scale.
+ * work: nb_g1_grad_work_bytes(count) bytes, 16-byte aligned. */
+long long nb_g1_grad_work_bytes(int count);
+int nb_g1_grad_sumsq(cudaStream_t stream, int count, const void* const* grads, const long long* sizes,
+                     const int* types, int zero_nonfinite, void* work, double* stats);
+int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
+                     const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
+                     double max_norm, double eps, const double* stats, float* norm, long long* bad);
+int nb_g1_grad_clip(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
+                    const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
+                    double max_norm, double eps, void* work, float* norm, long long* bad);
+
 #ifdef __cplusplus
 }
 #endif

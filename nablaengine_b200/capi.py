@@ -14,7 +14,9 @@ EXPORTS = ("nb_g1_sizes", "nb_g1_work_bytes", "nb_g1_upload", "nb_g1_forward", "
            "nb_g1_adjoint", "nb_g1_jacobian", "nb_g1_kinematics", "nb_g1_kinematics_vjp", "nb_g1_diag_count",
            "nb_g1_diag_forward", "nb_g1_diag_backward", "nb_g1_forward_noalloc", "nb_g1_last_forward",
            "nb_g1_launch", "nb_g1_tape_words", "nb_g1_forward_ex", "nb_g1_adjoint_ex", "nb_g1_jacobian_ex",
-           "nb_g1_diag_forward_ex")
+           "nb_g1_diag_forward_ex", "nb_g1_layer_norm_work_bytes", "nb_g1_layer_norm_forward",
+           "nb_g1_layer_norm_backward", "nb_g1_grad_work_bytes", "nb_g1_grad_sumsq", "nb_g1_grad_scale",
+           "nb_g1_grad_clip")
 ABI_VERSION = 4
 NQ, NV, NU, NBODY, MAXCON, NEFC = 36, 35, 29, 31, 64, 192
 
@@ -73,6 +75,18 @@ def load(path=None, build_if_missing=True):
         lib.nb_g1_jacobian_ex.restype = i32
         lib.nb_g1_diag_forward_ex.argtypes = lib.nb_g1_diag_forward.argtypes + [i32]
         lib.nb_g1_diag_forward_ex.restype = i32
+        f32, f64 = ctypes.c_float, ctypes.c_double
+        lib.nb_g1_layer_norm_work_bytes.argtypes, lib.nb_g1_layer_norm_work_bytes.restype = [i64, i64], i64
+        lib.nb_g1_layer_norm_forward.argtypes = [vp, i64, i64, i64, i32, vp, i32, vp, vp, f32, vp, vp, vp]
+        lib.nb_g1_layer_norm_forward.restype = i32
+        lib.nb_g1_layer_norm_backward.argtypes = [vp] + [i64] * 4 + [i32] + [vp] * 4 + [i32] + [vp] * 5
+        lib.nb_g1_layer_norm_backward.restype = i32
+        lib.nb_g1_grad_work_bytes.argtypes, lib.nb_g1_grad_work_bytes.restype = [i32], i64
+        lib.nb_g1_grad_sumsq.argtypes, lib.nb_g1_grad_sumsq.restype = [vp, i32, vp, vp, vp, i32, vp, vp], i32
+        lib.nb_g1_grad_scale.argtypes = [vp, i32] + [vp] * 5 + [i32, f64, f64] + [vp] * 3
+        lib.nb_g1_grad_scale.restype = i32
+        lib.nb_g1_grad_clip.argtypes = [vp, i32] + [vp] * 5 + [i32, f64, f64] + [vp] * 3
+        lib.nb_g1_grad_clip.restype = i32
         sizes = (ctypes.c_longlong * 8)()
         lib.nb_g1_sizes(sizes)
         want = (NQ, NV, NU, NBODY, MAXCON, NEFC)
