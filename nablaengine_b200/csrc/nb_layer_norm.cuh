@@ -1,81 +1,500 @@
 // Layer norm over the last dimension (N columns, M rows), forward and backward.
 //   mean = sum x / N, var = sum (x - mean)^2 / N, rstd = (var + eps)^(-1/2), xh = (x - mean) rstd, y = xh w + b
 //   h = g w, c1 = sum h / N, c2 = sum h xh / N, gx = rstd (h - c1 - xh c2), gw = sum_rows g xh, gb = sum_rows g
-// Sums are float32; the variance is taken from the deviations (a second pass), not from sum x^2.
+// Sums are float32; the variance is taken from the deviations (a second pass over registers), not from sum x^2.
+//
+// A block takes tiles of rows in turn. The tiles come through a ring of up to four stages in shared memory, filled by
+// asynchronous copies, so loads are in flight while a tile is worked on, and a dense x is copied in 16-byte pieces
+// whatever its width: a tile is one span of memory, rounded out to whole pieces, and a row starts where it starts.
+// From shared memory a row goes to the registers of `lanes` threads (8 to 1024, a power of two), EPT values each. A
+// thread keeps the same columns for every row it takes, so the weight, the bias and the two column sums of the backward
+// stay in its registers too. Rows that do not fit take the row-in-memory kernels at the end.
 #pragma once
+#include <cstdint>
 #include "nb_values.cuh"
 
 namespace nbtrain {
 
-constexpr int LN_WARPS = 8;     // warps (rows) per block
-constexpr int LN_PARTS = 256;   // partial column sums at most
+constexpr int LN_MAX_COLS = 16384;  // the widest row held in registers
+// The threads of a block and the blocks per SM for rows of `lanes` lanes of e-byte values, as measured. Forward: one
+// large block (131072 x 512 float32 88 us, 6100 GB/s, against 97 in two of half the size; 262144 x 512 bfloat16 88
+// against 97), but two for 16-bit rows that are spread over several warps, where one computes while the other waits for
+// its sums (131072 x 1024: 95 us against 108). Backward: one block for float32, which is bound by DRAM then
+// (131072 x 512: 128 us, 6300 GB/s, against 142 in two), two for 16 bits, bound by its instructions (131072 x 1024:
+// 133 us against 166).
+__host__ __device__ constexpr int ln_threads(int lanes, int e, bool backward) {
+  return lanes >= 512 ? lanes : !backward && (e == 4 || lanes <= 32) ? 512 : 256;
+}
+__host__ __device__ constexpr int ln_per_sm(int lanes, int e, bool backward) {
+  return ln_threads(lanes, e, backward) == 256 && !(backward && e == 4) ? 2 : 1;
+}
 
-// One warp per row, the row read three times (mean, variance, result).
-template <class T, class W>
-__global__ void __launch_bounds__(LN_WARPS * 32) k_ln_forward(long long rows, int cols, long long stride,
-                                                              const T* __restrict__ x, const W* __restrict__ weight,
-                                                              const W* __restrict__ bias, float eps,
-                                                              T* __restrict__ y, float* __restrict__ mean_out,
-                                                              float* __restrict__ rstd_out) {
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * LN_WARPS + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const T* xr = x + row * stride;
-  float s = 0.f;
-  for (int c = lane; c < cols; c += 32) s += to_f32(xr[c]);
-  const float mean = warp_sum(s) / cols;
-  s = 0.f;
-  for (int c = lane; c < cols; c += 32) {
-    const float d = to_f32(xr[c]) - mean;
-    s = fmaf(d, d, s);
+// How a tensor's rows lie: SPAN: dense rows from a 16-byte boundary; PIECES: every row a whole number of 16-byte
+// pieces from a 16-byte boundary; VALUES: anything else.
+enum LnRows { SPAN = 0, PIECES = 1, VALUES = 2 };
+
+// The tiles of a call: rows of a tile, the tile's bytes in a stage (per tensor) and a stage's bytes.
+struct LnTiles {
+  long long rows;
+  int cols, lanes, ept, per_tile, stages, tile_bytes, stage_bytes;
+};
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the newest n groups are complete (n: 0 to 3)
+__device__ __forceinline__ void copy_wait(int n) {
+  if (n == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+}
+
+// One tensor's rows on their way into the ring: a block's tiles one after the other.
+template <class T, int THREADS> struct LnFeed {
+  static constexpr int P = 16 / sizeof(T);
+  const T* next;  // the first row of the next tile
+  int kind, cols;
+  long long stride, step;  // in values: between rows, between the block's tiles
+  __device__ __forceinline__ LnFeed(const T* x, int kind, long long stride, const LnTiles& t, int cols)
+      : next(x + (long long)blockIdx.x * t.per_tile * stride),
+        kind(kind),
+        cols(cols),
+        stride(stride),
+        step((long long)gridDim.x * t.per_tile * stride) {}
+  // The byte at which the first row of the tile at p starts in its stage.
+  __device__ __forceinline__ int phase(const T* p) const {
+    return kind == SPAN ? (int)(reinterpret_cast<uintptr_t>(p) & 15) : 0;
   }
-  const float rstd = 1.f / sqrtf(warp_sum(s) / cols + eps);
-  for (int c = lane; c < cols; c += 32) {
-    float v = (to_f32(xr[c]) - mean) * rstd;
-    if (weight) v *= to_f32(weight[c]);
-    if (bias) v += to_f32(bias[c]);
-    y[row * cols + c] = from_f32<T>(v);
+  // Start copying the next tile's n rows into `dst` (16-byte aligned); `last`: the tensor ends with them.
+  __device__ __forceinline__ void fill(unsigned char* dst, int n, bool last) {
+    if (kind == SPAN) {
+      const int lead = phase(next), bytes = lead + n * cols * (int)sizeof(T);
+      const int pieces = last ? bytes >> 4 : (bytes + 15) >> 4;
+      const unsigned char* from = reinterpret_cast<const unsigned char*>(next) - lead;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < pieces; i += THREADS) copy_async16(dst + i * 16, from + i * 16);
+      if (last && (bytes & 15))  // the tensor's last values, less than a piece
+        for (int i = pieces * P + threadIdx.x; i < bytes / (int)sizeof(T); i += THREADS)
+          reinterpret_cast<T*>(dst)[i] = reinterpret_cast<const T*>(from)[i];
+    } else if (kind == PIECES) {
+      const int per_row = cols / P, pieces = per_row * n;
+      for (int i = threadIdx.x; i < pieces; i += THREADS) {
+        const int r = i / per_row;
+        copy_async16(dst + i * 16, next + r * stride + (i - r * per_row) * P);
+      }
+    } else {
+      for (int r = threadIdx.x >> 5; r < n; r += THREADS / 32) {
+        const T* from = next + r * stride;
+        T* to = reinterpret_cast<T*>(dst) + r * cols;
+        if (sizeof(T) == 4) {
+          for (int c = threadIdx.x & 31; c < cols; c += 32) copy_async4(to + c, from + c);
+        } else {
+#pragma unroll 8
+          for (int c = threadIdx.x & 31; c < cols; c += 32) to[c] = from[c];
+        }
+      }
+    }
+    next += step;
   }
-  if (lane == 0) {
-    mean_out[row] = mean;
-    rstd_out[row] = rstd;
+};
+
+// A block's tiles: the first row of the tile that is worked on, and of the one that is filled.
+struct LnTurn {
+  long long rows, row, fill_row, step;
+  int per_tile;
+  __device__ __forceinline__ explicit LnTurn(const LnTiles& t)
+      : rows(t.rows),
+        row((long long)blockIdx.x * t.per_tile),
+        fill_row(row),
+        step((long long)gridDim.x * t.per_tile),
+        per_tile(t.per_tile) {}
+  __device__ __forceinline__ int here(long long at) const {
+    return rows - at < per_tile ? (int)(rows - at) : per_tile;
+  }
+};
+
+// The LANES threads that share a row, and the sums of one or two floats over them: shuffles inside a warp, and for
+// wider rows one exchange through `slots` (two sets in turn, so one barrier is enough) under the group's own named
+// barrier. A thread holds the row's values i = 0 .. EPT - 1 at the columns (i / V * LANES + lane) * V + i % V, in pairs.
+template <int LANES> struct LnGroup {
+  static constexpr int WARPS = LANES / 32;
+  int lane, index;  // lane: the thread's place in its row's group; index: the group in the block
+  float2* slots;    // 2 x 32
+  int turn;
+  template <int N> __device__ __forceinline__ void sum(float (&v)[N]) {
+#pragma unroll
+    for (int m = (LANES < 32 ? LANES : 32) / 2; m > 0; m >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
+    if constexpr (LANES > 32) {
+      float2* s = slots + (turn & 1) * 32 + index * WARPS;
+      turn++;
+      if ((threadIdx.x & 31) == 0) s[lane >> 5] = make_float2(v[0], v[N - 1]);
+      asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "n"(LANES) : "memory");
+      const float2 o = s[threadIdx.x & (WARPS - 1)];
+      v[0] = o.x;
+      v[N - 1] = N == 1 ? o.x : o.y;
+#pragma unroll
+      for (int m = WARPS / 2; m > 0; m >>= 1)
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
+    }
+  }
+};
+
+template <int LANES, int V> __device__ __forceinline__ int ln_column(int lane, int i) {
+  return (i / V * LANES + lane) * V + i % V;
+}
+
+// A thread's values of a parameter, `absent` where there is none.
+template <int LANES, int EPT, int V>
+__device__ __forceinline__ void load_param(const void* p, int wtype, float absent, int cols, int lane, float2* out) {
+#pragma unroll
+  for (int i = 0; i < EPT; i++) {
+    const int c = ln_column<LANES, V>(lane, i);
+    float v = absent;
+    if (p && c < cols)
+      v = wtype == F32 ? static_cast<const float*>(p)[c]
+          : wtype == BF16 ? to_f32(static_cast<const __nv_bfloat16*>(p)[c])
+                          : to_f32(static_cast<const __half*>(p)[c]);
+    (i % 2 ? out[i / 2].y : out[i / 2].x) = v;
   }
 }
 
-// The input's gradient: one warp per row.
-template <class T, class W>
-__global__ void __launch_bounds__(LN_WARPS * 32) k_ln_backward_x(long long rows, int cols, long long gstride,
-                                                                 long long stride, const T* __restrict__ g,
-                                                                 const T* __restrict__ x,
-                                                                 const float* __restrict__ mean,
-                                                                 const float* __restrict__ rstd,
-                                                                 const W* __restrict__ weight, T* __restrict__ gx) {
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * LN_WARPS + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const T *xr = x + row * stride, *gr = g + row * gstride;
-  const float m = mean[row], r = rstd[row];
-  float c1 = 0.f, c2 = 0.f;
-  for (int c = lane; c < cols; c += 32) {
-    const float h = to_f32(gr[c]) * (weight ? to_f32(weight[c]) : 1.f);
-    c1 += h;
-    c2 = fmaf(h, (to_f32(xr[c]) - m) * r, c2);
+// A thread's values of a row, 0 beyond the last column.
+template <class T, int LANES, int EPT, int V, bool FULL>
+__device__ __forceinline__ void load_row(const T* row, int cols, int lane, float2* out) {
+  if constexpr (V == 1) {
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+      const int c = i * LANES + lane;
+      (i % 2 ? out[i / 2].y : out[i / 2].x) = c < cols ? to_f32(row[c]) : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPT / V; j++) {
+      const int c = (j * LANES + lane) * V;
+      load_pairs<T, V>(row + c, FULL || c < cols, out + j * V / 2);
+    }
   }
-  c1 = warp_sum(c1) / cols;
-  c2 = warp_sum(c2) / cols;
-  for (int c = lane; c < cols; c += 32) {
-    const float h = to_f32(gr[c]) * (weight ? to_f32(weight[c]) : 1.f);
-    gx[row * cols + c] = from_f32<T>((h - c1 - (to_f32(xr[c]) - m) * r * c2) * r);
+}
+
+template <class T, int LANES, int EPT, int V, bool FULL>
+__device__ __forceinline__ void store_row(T* row, int cols, int lane, const float2* v) {
+  if constexpr (V == 1) {
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+      const int c = i * LANES + lane;
+      if (c < cols) row[c] = from_f32<T>(i % 2 ? v[i / 2].y : v[i / 2].x);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPT / V; j++) {
+      const int c = (j * LANES + lane) * V;
+      if (FULL || c < cols) store_pairs<T, V>(row + c, v + j * V / 2);
+    }
+  }
+}
+
+// Set the places beyond the last column to 0.
+template <int LANES, int EPT, int V>
+__device__ __forceinline__ void clear_beyond(int cols, int lane, float2* v) {
+#pragma unroll
+  for (int i = 0; i < EPT; i++)
+    if (ln_column<LANES, V>(lane, i) >= cols) (i % 2 ? v[i / 2].y : v[i / 2].x) = 0.f;
+}
+
+// FULL: cols = LANES * EPT (no thread has a place beyond the last column)
+template <class T, int LANES, int EPT, int V, bool FULL>
+__global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm(LANES, sizeof(T), false))
+    k_ln_forward(LnTiles t, int kind, long long stride, const T* __restrict__ x, int wtype,
+                 const void* __restrict__ weight, const void* __restrict__ bias, float eps, T* __restrict__ y,
+                 float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float2 slots[64];
+  constexpr int THREADS = ln_threads(LANES, sizeof(T), false), GROUPS = THREADS / LANES, N2 = EPT / 2;
+  const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
+  LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
+  const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;  // the group's place in its warp
+  const float inv = 1.f / cols;
+  LnFeed<T, THREADS> feed(x, kind, stride, t, cols);
+  LnTurn turn(t);
+  auto fill = [&](int stage) {
+    if (turn.fill_row < turn.rows) {
+      const int n = turn.here(turn.fill_row);
+      feed.fill(ring + stage * t.stage_bytes, n, turn.fill_row + n == turn.rows);
+      turn.fill_row += turn.step;
+    }
+    copy_commit();
+  };
+  const T* at = feed.next;
+  T* out = y + turn.row * cols;
+  const long long out_step = turn.step * cols;
+  for (int s = 0; s + 1 < t.stages; s++) fill(s);
+  float2 w[N2], b[N2];
+  load_param<LANES, EPT, V>(weight, wtype, 1.f, cols, lane, w);
+  load_param<LANES, EPT, V>(bias, wtype, 0.f, cols, lane, b);
+  int stage = 0, free_stage = t.stages - 1;
+  for (; turn.row < turn.rows; turn.row += turn.step, at += feed.step, out += out_step) {
+    copy_wait(t.stages - 2);
+    __syncthreads();  // the tile is here, and nobody reads the stage of the tile before it any more
+    fill(free_stage);
+    const int n = turn.here(turn.row);
+    const T* rows = reinterpret_cast<const T*>(ring + stage * t.stage_bytes + feed.phase(at));
+    free_stage = stage;
+    stage = stage + 1 == t.stages ? 0 : stage + 1;
+    for (int r0 = g.index - shift; r0 < n; r0 += GROUPS) {  // (r0: the warp's first row)
+      const int r = r0 + shift;
+      float2 v[N2];
+      load_row<T, LANES, EPT, V, FULL>(rows + min(r, n - 1) * cols, cols, lane, v);
+      float2 a = v[0];
+#pragma unroll
+      for (int i = 1; i < N2; i++) a = add2(a, v[i]);
+      float s[1] = {a.x + a.y};
+      g.sum(s);
+      const float mean = s[0] * inv;
+#pragma unroll
+      for (int i = 0; i < N2; i++) v[i] = add2(v[i], both(-mean));
+      if (!FULL) clear_beyond<LANES, EPT, V>(cols, lane, v);
+      a = mul2(v[0], v[0]);
+#pragma unroll
+      for (int i = 1; i < N2; i++) a = fma2(v[i], v[i], a);
+      s[0] = a.x + a.y;
+      g.sum(s);
+      const float rstd = rsqrtf(fmaf(s[0], inv, eps));
+#pragma unroll
+      for (int i = 0; i < N2; i++) v[i] = fma2(mul2(v[i], both(rstd)), w[i], b[i]);
+      if (r < n) {
+        store_row<T, LANES, EPT, V, FULL>(out + r * cols, cols, lane, v);
+        if (lane < 2) (lane ? rstd_out : mean_out)[turn.row + r] = lane ? rstd : mean;
+      }
+    }
+  }
+}
+
+// part (gridDim.x, 2, cols), if wanted: the block's column sums of g xh and g
+// FULL: cols = LANES * EPT (no thread has a place beyond the last column)
+template <class T, int LANES, int EPT, int V, bool FULL>
+__global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(LANES, sizeof(T), true))
+    k_ln_backward(LnTiles t, int gkind, long long gstride, int kind, long long stride, const T* __restrict__ gy,
+                  const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd, int wtype,
+                  const void* __restrict__ weight, T* __restrict__ gx, float* __restrict__ part) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float2 slots[64];
+  constexpr int THREADS = ln_threads(LANES, sizeof(T), true), GROUPS = THREADS / LANES, N2 = EPT / 2;
+  const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
+  LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
+  const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;
+  const float inv = 1.f / cols;
+  LnFeed<T, THREADS> xfeed(x, kind, stride, t, cols), gfeed(gy, gkind, gstride, t, cols);
+  LnTurn turn(t);
+  auto fill = [&](int stage) {
+    if (turn.fill_row < turn.rows) {
+      unsigned char* to = ring + stage * t.stage_bytes;
+      const int n = turn.here(turn.fill_row);
+      const bool last = turn.fill_row + n == turn.rows;
+      xfeed.fill(to, n, last);
+      gfeed.fill(to + t.tile_bytes, n, last);
+      float* stats = reinterpret_cast<float*>(to + 2 * t.tile_bytes);
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        copy_async4(stats + i, mean + turn.fill_row + i);
+        copy_async4(stats + t.per_tile + i, rstd + turn.fill_row + i);
+      }
+      turn.fill_row += turn.step;
+    }
+    copy_commit();
+  };
+  const T *xat = xfeed.next, *gat = gfeed.next;
+  T* out = gx + turn.row * cols;
+  const long long out_step = turn.step * cols;
+  for (int s = 0; s + 1 < t.stages; s++) fill(s);
+  float2 w[N2], gw[N2], gb[N2];
+  load_param<LANES, EPT, V>(weight, wtype, 1.f, cols, lane, w);
+#pragma unroll
+  for (int i = 0; i < N2; i++) gw[i] = gb[i] = both(0.f);
+  int stage = 0, free_stage = t.stages - 1;
+  for (; turn.row < turn.rows; turn.row += turn.step, xat += xfeed.step, gat += gfeed.step, out += out_step) {
+    copy_wait(t.stages - 2);
+    __syncthreads();
+    fill(free_stage);
+    const int n = turn.here(turn.row);
+    const unsigned char* base = ring + stage * t.stage_bytes;
+    const T* xrows = reinterpret_cast<const T*>(base + xfeed.phase(xat));
+    const T* grows = reinterpret_cast<const T*>(base + t.tile_bytes + gfeed.phase(gat));
+    const float* stats = reinterpret_cast<const float*>(base + 2 * t.tile_bytes);
+    free_stage = stage;
+    stage = stage + 1 == t.stages ? 0 : stage + 1;
+    for (int r0 = g.index - shift; r0 < n; r0 += GROUPS) {
+      const int r = r0 + shift, at = min(r, n - 1);
+      float2 xh[N2], h[N2];
+      load_row<T, LANES, EPT, V, FULL>(xrows + at * cols, cols, lane, xh);
+      load_row<T, LANES, EPT, V, FULL>(grows + at * cols, cols, lane, h);
+      const float m = stats[at], rs = stats[t.per_tile + at];
+#pragma unroll
+      for (int i = 0; i < N2; i++) xh[i] = mul2(add2(xh[i], both(-m)), both(rs));
+      if (!FULL) clear_beyond<LANES, EPT, V>(cols, lane, xh);
+      if (r < n) {
+#pragma unroll
+        for (int i = 0; i < N2; i++) {
+          gw[i] = fma2(h[i], xh[i], gw[i]);
+          gb[i] = add2(gb[i], h[i]);
+        }
+      }
+      float2 c1 = both(0.f), c2 = both(0.f);
+#pragma unroll
+      for (int i = 0; i < N2; i++) {
+        h[i] = mul2(h[i], w[i]);
+        c1 = add2(c1, h[i]);
+        c2 = fma2(h[i], xh[i], c2);
+      }
+      float c[2] = {c1.x + c1.y, c2.x + c2.y};
+      g.sum(c);
+      if (!gx || r >= n) continue;
+      c1 = both(-c[0] * inv);
+      c2 = both(-c[1] * inv);
+#pragma unroll
+      for (int i = 0; i < N2; i++) h[i] = mul2(add2(fma2(xh[i], c2, h[i]), c1), both(rs));
+      store_row<T, LANES, EPT, V, FULL>(out + r * cols, cols, lane, h);
+    }
+  }
+  if (!part) return;
+  // the groups' column sums: over the groups of a warp by shuffles, then group by group through shared memory
+#pragma unroll
+  for (int m = LANES; m < 32; m <<= 1) {
+#pragma unroll
+    for (int i = 0; i < N2; i++) {
+      gw[i].x += __shfl_xor_sync(0xffffffffu, gw[i].x, m);
+      gw[i].y += __shfl_xor_sync(0xffffffffu, gw[i].y, m);
+      gb[i].x += __shfl_xor_sync(0xffffffffu, gb[i].x, m);
+      gb[i].y += __shfl_xor_sync(0xffffffffu, gb[i].y, m);
+    }
+  }
+  float* total = reinterpret_cast<float*>(ring);  // (2, cols), over the ring
+  constexpr int UNIT = LANES < 32 ? 32 : LANES, UNITS = THREADS / UNIT;
+  const int mine = threadIdx.x / UNIT;
+  float* sums = part + (long long)blockIdx.x * 2 * cols;
+  copy_wait(0);
+  for (int u = 0; u < UNITS; u++) {
+    __syncthreads();
+    if (u != mine || (LANES < 32 && (threadIdx.x & 31) >= LANES)) continue;
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+      const int c = ln_column<LANES, V>(lane, i);
+      if (c >= cols) continue;
+      float a = i % 2 ? gw[i / 2].y : gw[i / 2].x, d = i % 2 ? gb[i / 2].y : gb[i / 2].x;
+      if (u) a += total[c], d += total[cols + c];
+      if (u + 1 < UNITS) total[c] = a, total[cols + c] = d;
+      else sums[c] = a, sums[cols + c] = d;
+    }
+  }
+}
+
+// gw, gb = the sums of the blocks' column sums: 32 columns a block, 8 threads to a column
+template <class W>
+__global__ void __launch_bounds__(256) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
+                                                         W* __restrict__ gw, W* __restrict__ gb) {
+  __shared__ float s[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;  // 0 .. 2 cols: gw's columns, then gb's
+  float v = 0.f;
+  if (c < 2 * cols) {
+#pragma unroll 8
+    for (int p = warp; p < parts; p += 8) v += part[(long long)p * 2 * cols + c];
+  }
+  s[warp][lane] = v;
+  __syncthreads();
+  if (warp || c >= 2 * cols) return;
+#pragma unroll
+  for (int k = 1; k < 8; k++) v += s[k][lane];
+  if (c < cols) {
+    if (gw) gw[c] = from_f32<W>(v);
+  } else if (gb) {
+    gb[c - cols] = from_f32<W>(v);
+  }
+}
+
+// ---- rows that no ring holds: a block per row, the row read again from memory in each pass ---------------------
+__device__ __forceinline__ float wide_sum(float v) {
+  __shared__ float s[32];
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s[threadIdx.x & 31];
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+template <class T, class W>
+__global__ void __launch_bounds__(1024) k_ln_forward_wide(long long rows, int cols, long long stride,
+                                                          const T* __restrict__ x, const W* __restrict__ weight,
+                                                          const W* __restrict__ bias, float eps, T* __restrict__ y,
+                                                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * stride;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 1024) s += to_f32(xr[c]);
+    const float mean = wide_sum(s) / cols;
+    s = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 1024) {
+      const float d = to_f32(xr[c]) - mean;
+      s = fmaf(d, d, s);
+    }
+    const float rstd = rsqrtf(wide_sum(s) / cols + eps);
+    for (int c = threadIdx.x; c < cols; c += 1024) {
+      float v = (to_f32(xr[c]) - mean) * rstd;
+      if (weight) v *= to_f32(weight[c]);
+      if (bias) v += to_f32(bias[c]);
+      y[row * cols + c] = from_f32<T>(v);
+    }
+    if (threadIdx.x == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+  }
+}
+
+template <class T, class W>
+__global__ void __launch_bounds__(1024) k_ln_backward_wide(long long rows, int cols, long long gstride,
+                                                           long long stride, const T* __restrict__ g,
+                                                           const T* __restrict__ x, const float* __restrict__ mean,
+                                                           const float* __restrict__ rstd,
+                                                           const W* __restrict__ weight, T* __restrict__ gx) {
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T *xr = x + row * stride, *gr = g + row * gstride;
+    const float m = mean[row], r = rstd[row];
+    float c1 = 0.f, c2 = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 1024) {
+      const float h = to_f32(gr[c]) * (weight ? to_f32(weight[c]) : 1.f);
+      c1 += h;
+      c2 = fmaf(h, (to_f32(xr[c]) - m) * r, c2);
+    }
+    c1 = wide_sum(c1) / cols;
+    c2 = wide_sum(c2) / cols;
+    for (int c = threadIdx.x; c < cols; c += 1024) {
+      const float h = to_f32(gr[c]) * (weight ? to_f32(weight[c]) : 1.f);
+      gx[row * cols + c] = from_f32<T>((h - c1 - (to_f32(xr[c]) - m) * r * c2) * r);
+    }
   }
 }
 
 // Column sums of g xh and g over part_rows rows per block row, one thread per column: part (parts, 2, cols).
 template <class T>
-__global__ void __launch_bounds__(128) k_ln_backward_part(long long rows, int cols, long long gstride,
-                                                          long long stride, const T* __restrict__ g,
-                                                          const T* __restrict__ x, const float* __restrict__ mean,
-                                                          const float* __restrict__ rstd, long long part_rows,
-                                                          float* __restrict__ part) {
+__global__ void __launch_bounds__(128) k_ln_backward_wide_part(long long rows, int cols, long long gstride,
+                                                               long long stride, const T* __restrict__ g,
+                                                               const T* __restrict__ x,
+                                                               const float* __restrict__ mean,
+                                                               const float* __restrict__ rstd, long long part_rows,
+                                                               float* __restrict__ part) {
   const int c = blockIdx.x * 128 + threadIdx.x;
   if (c >= cols) return;
   const long long r0 = blockIdx.y * part_rows, r1 = r0 + part_rows < rows ? r0 + part_rows : rows;
@@ -87,20 +506,6 @@ __global__ void __launch_bounds__(128) k_ln_backward_part(long long rows, int co
   }
   part[((long long)blockIdx.y * 2 + 0) * cols + c] = gw;
   part[((long long)blockIdx.y * 2 + 1) * cols + c] = gb;
-}
-
-template <class W>
-__global__ void __launch_bounds__(128) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
-                                                         W* __restrict__ gw, W* __restrict__ gb) {
-  const int c = blockIdx.x * 128 + threadIdx.x;
-  if (c >= cols) return;
-  float w = 0.f, b = 0.f;
-  for (int p = 0; p < parts; p++) {
-    w += part[((long long)p * 2 + 0) * cols + c];
-    b += part[((long long)p * 2 + 1) * cols + c];
-  }
-  if (gw) gw[c] = from_f32<W>(w);
-  if (gb) gb[c] = from_f32<W>(b);
 }
 
 }  // namespace nbtrain

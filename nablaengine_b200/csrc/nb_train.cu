@@ -7,55 +7,19 @@
 #include <cstdint>
 #include <new>
 #include "nb_grad_norm.cuh"
-#include "nb_layer_norm.cuh"
+#include "nb_layer_norm_call.h"
 
 using namespace nbtrain;
 
 namespace {
 
-// ---- layer norm ---------------------------------------------------------------------------------------------------
+// ---- arguments ------------------------------------------------------------------------------------------------------
 bool ln_args_ok(long long rows, long long cols, long long stride, int dtype, int wtype) {
   return rows >= 0 && cols >= 1 && cols <= INT_MAX / 4 && stride >= 0 && dtype_ok(dtype) &&
-         (wtype == F32 || wtype == dtype) && rows <= (long long)INT_MAX * LN_WARPS;
+         (wtype == F32 || wtype == dtype);
 }
 
 bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) == 0; }
-
-int ln_parts(long long rows) { return (int)std::min<long long>(LN_PARTS, (rows + 63) / 64); }
-
-template <class T, class W>
-int ln_forward(cudaStream_t stream, long long rows, int cols, long long stride, const void* x, const void* weight,
-               const void* bias, float eps, void* y, float* mean, float* rstd) {
-  k_ln_forward<T, W><<<(unsigned)((rows + LN_WARPS - 1) / LN_WARPS), LN_WARPS * 32, 0, stream>>>(
-      rows, cols, stride, static_cast<const T*>(x), static_cast<const W*>(weight), static_cast<const W*>(bias), eps,
-      static_cast<T*>(y), mean, rstd);
-  return (int)cudaGetLastError();
-}
-
-template <class T, class W>
-int ln_backward(cudaStream_t stream, long long rows, int cols, long long gstride, long long stride, const void* g,
-                const void* x, const float* mean, const float* rstd, const void* weight, void* gx, void* gw, void* gb,
-                float* part) {
-  const T *gp = static_cast<const T*>(g), *xp = static_cast<const T*>(x);
-  if (gx && rows)
-    k_ln_backward_x<T, W><<<(unsigned)((rows + LN_WARPS - 1) / LN_WARPS), LN_WARPS * 32, 0, stream>>>(
-        rows, cols, gstride, stride, gp, xp, mean, rstd, static_cast<const W*>(weight), static_cast<T*>(gx));
-  if (gw || gb) {
-    const int parts = ln_parts(rows), blocks = (cols + 127) / 128;
-    if (parts)
-      k_ln_backward_part<T><<<dim3(blocks, parts), 128, 0, stream>>>(rows, cols, gstride, stride, gp, xp, mean, rstd,
-                                                                      (rows + parts - 1) / parts, part);
-    k_ln_backward_sum<W><<<blocks, 128, 0, stream>>>(parts, cols, part, static_cast<W*>(gw), static_cast<W*>(gb));
-  }
-  return (int)cudaGetLastError();
-}
-
-// calls f with the value types of x and of the parameters
-template <class F> int with_types(int dtype, int wtype, F f) {
-  if (dtype == F32) return f(float(), float());
-  if (dtype == BF16) return wtype == F32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
-  return wtype == F32 ? f(__half(), float()) : f(__half(), __half());
-}
 
 // ---- the gradient list ----------------------------------------------------------------------------------------------
 bool grads_ok(int count, const void* const* in, const long long* sizes, const int* types) {
@@ -154,7 +118,7 @@ extern "C" {
 
 long long nb_g1_layer_norm_work_bytes(long long rows, long long cols) {
   if (rows < 0 || cols < 1 || cols > INT_MAX / 4) return -1;
-  return (long long)ln_parts(rows) * 2 * cols * 4;
+  return ln_max_parts(rows, (int)cols) * 2 * cols * 4;
 }
 
 int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols, long long stride, int dtype,
@@ -166,9 +130,8 @@ int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols
   if (!x || !y || !mean || !rstd || !aligned(x, dtype) || !aligned(y, dtype) || !aligned(weight, wtype) ||
       !aligned(bias, wtype))
     return (int)cudaErrorInvalidValue;
-  return with_types(dtype, wtype, [&](auto t, auto w) {
-    return ln_forward<decltype(t), decltype(w)>(stream, rows, (int)cols, stride, x, weight, bias, eps, y, mean, rstd);
-  });
+  const LnForward a = {stream, rows, (int)cols, stride, x, wtype, weight, bias, eps, y, mean, rstd};
+  return dtype == F32 ? ln_forward<float>(a) : dtype == BF16 ? ln_forward<__nv_bfloat16>(a) : ln_forward<__half>(a);
 }
 
 int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long cols, long long g_stride,
@@ -180,10 +143,10 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
       !aligned(g_x, dtype) || !aligned(weight, wtype) || !aligned(g_weight, wtype) || !aligned(g_bias, wtype))
     return (int)cudaErrorInvalidValue;
   if (rows && (g_weight || g_bias) && !work) return (int)cudaErrorInvalidValue;
-  return with_types(dtype, wtype, [&](auto t, auto w) {
-    return ln_backward<decltype(t), decltype(w)>(stream, rows, (int)cols, g_stride, stride, g_y, x, mean, rstd, weight,
-                                                 g_x, g_weight, g_bias, static_cast<float*>(work));
-  });
+  const LnBackward a = {stream, rows, (int)cols, g_stride, stride, g_y, x, mean, rstd,
+                        wtype, weight, g_x, g_weight, g_bias, static_cast<float*>(work)};
+  return dtype == F32 ? ln_backward<float>(a) : dtype == BF16 ? ln_backward<__nv_bfloat16>(a)
+                                                              : ln_backward<__half>(a);
 }
 
 long long nb_g1_grad_work_bytes(int count) {
