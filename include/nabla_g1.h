@@ -202,7 +202,7 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
  * counts sizes (each tensor dense; 0 allowed), value types. S = the sum of all squares, in 64 bits; bad = the number
  * of non-finite values. zero_nonfinite: those count as 0 in S and are written as 0; otherwise they take part as the
  * arithmetic has them (S infinite or NaN).
- *   sumsq: stats (2 doubles) = S, bad; ranks that share a model add theirs up before the next call.
+ *   sumsq: stats (2 doubles, 16-byte aligned) = S, bad; ranks that share a model add theirs up before the next call.
  *   scale: c = min(1, max_norm / (sqrt(S) + eps)), outs[i] = c grads[i] in type out_types[i]; norm = sqrt(S) and bad,
  *     each where not NULL. An output may be its own gradient (same address and type); outputs that overlap anything
  *     else are refused. outs NULL: norm and bad alone.

@@ -1,102 +1,168 @@
 // The global norm of a list of tensors and the list times the clip coefficient:
 //   S = sum g^2 over every value of every tensor, norm = sqrt(S), c = min(1, max_norm / (norm + eps)), out = c g
-// S is summed in 64 bits, so neither a gradient of 1e30 overflows it nor one of 1e-30 vanishes from it, and in a fixed
-// order (one partial sum per block, no atomics), so results repeat bit for bit. Non-finite values are counted; with
-// `zero` they count as 0 in S and in out.
+// Non-finite values are counted; with `zero` they count as 0 in S and in out.
+//
+// S is held in 64 bits, so neither a gradient of 1e30 overflows it nor one of 1e-30 vanishes from it. Eight squares at a
+// time are summed in float32 first; where that sum is not between 2^-100 and the largest float (an overflow, values that
+// vanish, a non-finite one) the eight are taken again one by one in 64 bits. Every block writes one partial sum and the
+// next kernel's blocks add them all up, each for itself, in the same order: no atomics, the same bits every time.
+//
+// Both passes are bound by memory. The tensors are cut into chunks that the blocks take in turn, in the first pass from
+// the first chunk on and in the second from the last one back, so that the second finds in the second-level cache
+// what the first read last.
 #pragma once
+#include <cstdint>
 #include "nb_values.cuh"
 
 namespace nbtrain {
 
 constexpr int GN_THREADS = 256;
-constexpr int GN_CHUNK = 8192;     // values of one tensor that a block takes at a time
-constexpr int GN_MAX_BLOCKS = 1184;  // partial sums of a launch (8 blocks for each of the 148 SMs)
-constexpr int GN_TENSORS = 96;     // tensors of one launch (their table travels as a kernel argument)
+constexpr int GN_BLOCKS = 4 * SMS;  // blocks of a launch at most, and its partial sums
+constexpr int GN_FEW = 96, GN_MANY = 960;  // tensors of one launch (their table travels as a kernel argument)
+constexpr int GN_UNROLL = 4;  // 16-byte loads in flight per thread
 
+// One tensor: its values from the first 16-byte boundary on (`lead` values in) are cut into chunks.
 struct GradEntry {
   const void* in;
   void* out;
   long long n;
   int first;  // the tensor's first chunk in the launch
-  short in_type, out_type;
+  unsigned char in_type, out_type, lead, vectors;  // vectors: out takes whole pieces where in gives them
 };
-struct GradTable {
-  int count, chunks;
-  GradEntry t[GN_TENSORS];
+template <int N> struct GradTable {
+  int count, chunks, chunk;  // chunk: values of a chunk
+  GradEntry t[N];
 };
 
-__device__ __forceinline__ float load_value(const void* p, int type, long long i) {
-  if (type == BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
-  if (type == F16) return to_f32(static_cast<const __half*>(p)[i]);
-  return static_cast<const float*>(p)[i];
-}
-__device__ __forceinline__ void store_value(void* p, int type, long long i, float v) {
-  if (type == BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
-  else if (type == F16) static_cast<__half*>(p)[i] = from_f32<__half>(v);
-  else static_cast<float*>(p)[i] = v;
-}
-
-// The tensor of chunk `c`: the last one whose first chunk is at most c.
-__device__ __forceinline__ int tensor_of_chunk(const GradTable& t, int c) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.t[mid].first <= c) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+// The values [first, first + n) of the tensor `e` that chunk c of a table is, without the lead.
+struct GradPart {
+  long long first;
+  int n;
+};
+template <int N> __device__ __forceinline__ GradPart grad_part(const GradTable<N>& t, const GradEntry& e, int c) {
+  const long long first = e.lead + (long long)(c - e.first) * t.chunk, left = e.n - first;
+  return {first, (int)(left < t.chunk ? left : t.chunk)};
 }
 
-// A block's sum of a double per thread (the result at thread 0).
-__device__ __forceinline__ double block_sum(double v) {
-  __shared__ double s[GN_THREADS / 32];
+__device__ __forceinline__ void add_value(float v, int zero, double& s, double& bad) {
+  const bool finite = isfinite(v);
+  if (!finite) bad += 1.0;
+  if (finite || !zero) s = fma((double)v, (double)v, s);
+}
+// eight values (four pairs)
+__device__ __forceinline__ void add_eight(const float2* v, int zero, double& s, double& bad) {
+  float2 q = mul2(v[0], v[0]);
+  q = fma2(v[1], v[1], q);
+  q = fma2(v[2], v[2], q);
+  q = fma2(v[3], v[3], q);
+  const float sum = q.x + q.y;
+  if (sum >= 0x1p-100f && sum <= 3.4e38f) {
+    s += (double)sum;
+  } else {
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-  __syncthreads();
+    for (int i = 0; i < 4; i++) {
+      add_value(v[i].x, zero, s, bad);
+      add_value(v[i].y, zero, s, bad);
+    }
+  }
+}
+
+template <class T> __device__ __forceinline__ void unpack_piece(uint4 u, float2* v) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  } else {
+    v[0] = unpack2<T>(u.x), v[1] = unpack2<T>(u.y), v[2] = unpack2<T>(u.z), v[3] = unpack2<T>(u.w);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void sumsq_part(const GradEntry& e, GradPart part, int zero, double& s, double& bad) {
+  constexpr int P = 16 / sizeof(T), STEP = GN_THREADS * GN_UNROLL;
+  const T* base = static_cast<const T*>(e.in);
+  if (part.first == e.lead)
+    for (int i = threadIdx.x; i < min((long long)e.lead, e.n); i += GN_THREADS)
+      add_value(to_f32(base[i]), zero, s, bad);
+  if (part.n <= 0) return;
+  const uint4* from = reinterpret_cast<const uint4*>(base + part.first);
+  const int pieces = part.n / P;
+  int i = threadIdx.x;
+  for (; i + STEP - GN_THREADS < pieces; i += STEP) {
+    uint4 u[GN_UNROLL];
+#pragma unroll
+    for (int k = 0; k < GN_UNROLL; k++) u[k] = from[i + k * GN_THREADS];
+#pragma unroll
+    for (int k = 0; k < GN_UNROLL; k += P == 4 ? 2 : 1) {
+      float2 v[4];
+      unpack_piece<T>(u[k], v);
+      if constexpr (P == 4) unpack_piece<T>(u[k + 1], v + 2);
+      add_eight(v, zero, s, bad);
+    }
+  }
+  for (; i < pieces; i += GN_THREADS) {
+    float2 v[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+    unpack_piece<T>(from[i], v);
+    add_eight(v, zero, s, bad);
+  }
+  for (int k = pieces * P + threadIdx.x; k < part.n; k += GN_THREADS)
+    add_value(to_f32(base[part.first + k]), zero, s, bad);
+}
+
+// Sums over the block of a double per thread (the result at thread 0).
+__device__ __forceinline__ double2 block_sum(double2 v) {
+  __shared__ double2 s[GN_THREADS / 32];
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, m);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, m);
+  }
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x == 0)
-    for (int w = 1; w < GN_THREADS / 32; w++) v += s[w];
+    for (int w = 1; w < GN_THREADS / 32; w++) v.x += s[w].x, v.y += s[w].y;
   return v;
 }
 
-// part[2 (base + block)] = the block's sum of squares, [.. + 1] = its non-finite values
-__global__ void __launch_bounds__(GN_THREADS) k_grad_sumsq(const __grid_constant__ GradTable t, int zero, int base,
-                                                           double* __restrict__ part) {
+// part[base + block] = the block's sum of squares and its non-finite values
+template <int N>
+__global__ void __launch_bounds__(GN_THREADS) k_grad_sumsq(const __grid_constant__ GradTable<N> t, int zero, int base,
+                                                           double2* __restrict__ part) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   double s = 0.0, bad = 0.0;
+  int i = 0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const GradEntry& e = t.t[tensor_of_chunk(t, c)];
-    const long long i0 = (long long)(c - e.first) * GN_CHUNK;
-    const int n = (int)(e.n - i0 < GN_CHUNK ? e.n - i0 : GN_CHUNK);
-    for (int i = threadIdx.x; i < n; i += GN_THREADS) {
-      const float v = load_value(e.in, e.in_type, i0 + i);
-      const bool finite = isfinite(v);
-      if (!finite) bad += 1.0;
-      if (finite || !zero) s = fma((double)v, (double)v, s);
-    }
+    while (i + 1 < t.count && t.t[i + 1].first <= c) i++;
+    const GradEntry& e = t.t[i];
+    const GradPart p = grad_part(t, e, c);
+    if (e.in_type == F32) sumsq_part<float>(e, p, zero, s, bad);
+    else if (e.in_type == BF16) sumsq_part<__nv_bfloat16>(e, p, zero, s, bad);
+    else sumsq_part<__half>(e, p, zero, s, bad);
   }
-  s = block_sum(s);
-  bad = block_sum(bad);
-  if (threadIdx.x == 0) {
-    part[2 * (base + blockIdx.x)] = s;
-    part[2 * (base + blockIdx.x) + 1] = bad;
-  }
+  const double2 r = block_sum(make_double2(s, bad));
+  if (threadIdx.x == 0) part[base + blockIdx.x] = r;
 }
 
-// stats = the partial sums' sums (one block)
-__global__ void __launch_bounds__(GN_THREADS) k_grad_finish(int parts, const double* __restrict__ part,
-                                                            double* __restrict__ stats) {
-  double s = 0.0, bad = 0.0;
-  for (int i = threadIdx.x; i < parts; i += GN_THREADS) {
-    s += part[2 * i];
-    bad += part[2 * i + 1];
-  }
-  s = block_sum(s);
-  bad = block_sum(bad);
-  if (threadIdx.x == 0) {
-    stats[0] = s;
-    stats[1] = bad;
-  }
+// The sum of all partial sums, for every thread of the block.
+__device__ __forceinline__ double2 sum_parts(int parts, const double2* part) {
+  __shared__ double2 total;
+  double2 v = make_double2(0.0, 0.0);
+  for (int i = threadIdx.x; i < parts; i += GN_THREADS) v.x += part[i].x, v.y += part[i].y;
+  v = block_sum(v);
+  if (threadIdx.x == 0) total = v;
+  __syncthreads();
+  return total;
+}
+
+// The results alone (one block), each where wanted.
+__global__ void __launch_bounds__(GN_THREADS) k_grad_finish(int parts, const double2* __restrict__ part,
+                                                            double2* __restrict__ stats, float* __restrict__ norm,
+                                                            long long* __restrict__ bad) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double2 v = sum_parts(parts, part);
+  if (threadIdx.x) return;
+  if (stats) *stats = v;
+  if (norm) *norm = (float)sqrt(v.x);
+  if (bad) *bad = (long long)v.y;
 }
 
 __device__ __forceinline__ float clip_coefficient(double sumsq, double max_norm, double eps) {
@@ -104,24 +170,87 @@ __device__ __forceinline__ float clip_coefficient(double sumsq, double max_norm,
   return d <= max_norm ? 1.f : (float)(max_norm / d);  // (a NaN norm gives NaN, an infinite one 0)
 }
 
-__global__ void k_grad_result(const double* __restrict__ stats, float* __restrict__ norm, long long* __restrict__ bad) {
-  if (norm) *norm = (float)sqrt(stats[0]);
-  if (bad) *bad = (long long)stats[1];
+// c v; where non-finite values count as 0 and there are any, those are 0
+__device__ __forceinline__ float clip_value(float v, float c, bool clean) {
+  return clean && !isfinite(v) ? 0.f : v * c;
 }
 
-__global__ void __launch_bounds__(GN_THREADS) k_grad_scale(const __grid_constant__ GradTable t,
-                                                           const double* __restrict__ stats, double max_norm,
-                                                           double eps, int zero) {
-  const float coef = clip_coefficient(stats[0], max_norm, eps);
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const GradEntry& e = t.t[tensor_of_chunk(t, c)];
-    const long long i0 = (long long)(c - e.first) * GN_CHUNK;
-    const int n = (int)(e.n - i0 < GN_CHUNK ? e.n - i0 : GN_CHUNK);
-    for (int i = threadIdx.x; i < n; i += GN_THREADS) {
-      float v = load_value(e.in, e.in_type, i0 + i);
-      if (zero && !isfinite(v)) v = 0.f;
-      store_value(e.out, e.out_type, i0 + i, v * coef);
+template <class O, int P> __device__ __forceinline__ void store_piece(O* p, const float2* v) {
+  if constexpr (P * sizeof(O) == 32) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
+    __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[2].x, v[2].y, v[3].x, v[3].y));
+  } else if constexpr (sizeof(O) == 4) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
+  } else if constexpr (P == 8) {
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack2<O>(v[0]), pack2<O>(v[1]), pack2<O>(v[2]), pack2<O>(v[3])));
+  } else {
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack2<O>(v[0]), pack2<O>(v[1])));
+  }
+}
+
+template <class T, class O>
+__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, float coef, bool clean) {
+  constexpr int P = 16 / sizeof(T), STEP = GN_THREADS * GN_UNROLL;
+  const T* base = static_cast<const T*>(e.in);
+  O* out = static_cast<O*>(e.out);
+  auto one = [&](long long i) { out[i] = from_f32<O>(clip_value(to_f32(base[i]), coef, clean)); };
+  if (part.first == e.lead)
+    for (int i = threadIdx.x; i < min((long long)e.lead, e.n); i += GN_THREADS) one(i);
+  if (part.n <= 0) return;
+  const uint4* from = reinterpret_cast<const uint4*>(base + part.first);
+  O* to = out + part.first;
+  const int pieces = e.vectors ? part.n / P : 0;
+  auto piece = [&](int at, uint4 u) {
+    float2 v[P / 2];
+    unpack_piece<T>(u, v);
+#pragma unroll
+    for (int k = 0; k < P / 2; k++) {
+      if (clean) v[k] = make_float2(isfinite(v[k].x) ? v[k].x : 0.f, isfinite(v[k].y) ? v[k].y : 0.f);
+      v[k] = mul2(v[k], both(coef));
     }
+    store_piece<O, P>(to + (long long)at * P, v);
+  };
+  int i = threadIdx.x;
+  for (; i + STEP - GN_THREADS < pieces; i += STEP) {
+    uint4 u[GN_UNROLL];
+#pragma unroll
+    for (int k = 0; k < GN_UNROLL; k++) u[k] = __ldcs(from + i + k * GN_THREADS);
+#pragma unroll
+    for (int k = 0; k < GN_UNROLL; k++) piece(i + k * GN_THREADS, u[k]);
+  }
+  for (; i < pieces; i += GN_THREADS) piece(i, __ldcs(from + i));
+  for (int k = pieces * P + threadIdx.x; k < part.n; k += GN_THREADS) one(part.first + k);
+}
+
+template <class T>
+__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, float coef, bool clean) {
+  if (e.out_type == F32) scale_part<T, float>(e, part, coef, clean);
+  else if (e.out_type == BF16) scale_part<T, __nv_bfloat16>(e, part, coef, clean);
+  else scale_part<T, __half>(e, part, coef, clean);
+}
+
+template <int N>
+__global__ void __launch_bounds__(GN_THREADS) k_grad_scale(const __grid_constant__ GradTable<N> t, int parts,
+                                                           const double2* __restrict__ part, double max_norm,
+                                                           double eps, int zero, float* __restrict__ norm,
+                                                           long long* __restrict__ bad) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double2 stats = sum_parts(parts, part);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (norm) *norm = (float)sqrt(stats.x);
+    if (bad) *bad = (long long)stats.y;
+  }
+  const float coef = clip_coefficient(stats.x, max_norm, eps);
+  const bool clean = zero && stats.y > 0.0;
+  int i = t.count - 1;
+  for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+    while (t.t[i].first > c) i--;
+    const GradEntry& e = t.t[i];
+    if (coef == 1.f && !clean && e.in == e.out) continue;  // (in place, and every value stays as it is)
+    const GradPart p = grad_part(t, e, c);
+    if (e.in_type == F32) scale_part<float>(e, p, coef, clean);
+    else if (e.in_type == BF16) scale_part<__nv_bfloat16>(e, p, coef, clean);
+    else scale_part<__half>(e, p, coef, clean);
   }
 }
 

@@ -64,53 +64,111 @@ int outs_error(int count, const void* const* in, void* const* out, const long lo
   return err;
 }
 
-int grad_launches(int count) { return (count + GN_TENSORS - 1) / GN_TENSORS; }
+int grad_launches(int count) { return (count + GN_MANY - 1) / GN_MANY; }
 
-// The table of tensors [i0, i0 + GN_TENSORS) and its launch's blocks.
-int fill_table(GradTable& t, int i0, int count, const void* const* in, void* const* out, const long long* sizes,
+// The table of the tensors from i0 on, as many as it takes; returns its launch's blocks.
+template <int N>
+int fill_table(GradTable<N>& t, int i0, int count, const void* const* in, void* const* out, const long long* sizes,
                const int* types, const int* out_types) {
+  const int i1 = std::min(count, i0 + N);
+  long long total = 0, chunks = 0;
+  for (int i = i0; i < i1; i++) total += sizes[i];
+  // chunks of 2048 to 16384 values: about one for each block where the tensors are small
+  t.chunk = 2048;
+  while (t.chunk < 16384 && total > (long long)t.chunk * GN_BLOCKS) t.chunk *= 2;
   t.count = 0;
-  long long chunks = 0;
-  for (int i = i0; i < count && i < i0 + GN_TENSORS; i++) {
+  for (int i = i0; i < i1; i++) {
     if (sizes[i] == 0) continue;
     GradEntry& e = t.t[t.count++];
-    e = {in[i],       out ? out[i] : nullptr, sizes[i],
-         (int)chunks, (short)types[i],        (short)(out ? out_types[i] : types[i])};
-    chunks += (sizes[i] + GN_CHUNK - 1) / GN_CHUNK;
+    const int es = dtype_bytes(types[i]);
+    const uintptr_t a = reinterpret_cast<uintptr_t>(in[i]);
+    e.in = in[i];
+    e.out = out ? out[i] : nullptr;
+    e.n = sizes[i];
+    e.first = (int)chunks;
+    e.in_type = (unsigned char)types[i];
+    e.out_type = (unsigned char)(out ? out_types[i] : types[i]);
+    e.lead = (unsigned char)((16 - a % 16) % 16 / es);
+    const int os = dtype_bytes(e.out_type);
+    e.vectors = (reinterpret_cast<uintptr_t>(e.out) + (uintptr_t)e.lead * os) % std::min(16, 16 / es * os) == 0;
+    chunks += std::max<long long>(1, (sizes[i] - e.lead + t.chunk - 1) / t.chunk);
     if (chunks > INT_MAX / 2) return -1;
   }
   t.chunks = (int)chunks;
-  return (int)std::min<long long>(chunks, GN_MAX_BLOCKS);
+  return (int)std::min<long long>(chunks, GN_BLOCKS);
 }
 
-int grad_sumsq(cudaStream_t stream, int count, const void* const* grads, const long long* sizes, const int* types,
-               int zero, double* part, double* stats) {
-  GradTable t;
-  int parts = 0;
-  for (int i0 = 0; i0 < count; i0 += GN_TENSORS) {
-    const int blocks = fill_table(t, i0, count, grads, nullptr, sizes, types, nullptr);
+// Launch a kernel that may start while the one before it in the stream ends (it waits for it before its first access).
+template <class... P, class... A>
+int launch_after(cudaStream_t stream, int blocks, void (*kernel)(P...), A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(GN_THREADS);
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
+struct GradList {
+  int count;
+  const void* const* in;
+  void* const* out;
+  const long long* sizes;
+  const int *types, *out_types;
+  int zero;
+};
+
+// The partial sums of the list into `part`; sets their number.
+template <int N> int grad_sumsq(cudaStream_t stream, const GradList& g, double2* part, int* parts) {
+  GradTable<N> t;
+  *parts = 0;
+  for (int i0 = 0; i0 < g.count; i0 += N) {
+    const int blocks = fill_table(t, i0, g.count, g.in, nullptr, g.sizes, g.types, nullptr);
     if (blocks < 0) return cudaErrorInvalidValue;
     if (!blocks) continue;
-    k_grad_sumsq<<<blocks, GN_THREADS, 0, stream>>>(t, zero, parts, part);
-    parts += blocks;
+    k_grad_sumsq<N><<<blocks, GN_THREADS, 0, stream>>>(t, g.zero, *parts, part);
+    *parts += blocks;
   }
-  k_grad_finish<<<1, GN_THREADS, 0, stream>>>(parts, part, stats);
   return (int)cudaGetLastError();
+}
+int grad_sumsq(cudaStream_t stream, const GradList& g, double2* part, int* parts) {
+  return g.count <= GN_FEW ? grad_sumsq<GN_FEW>(stream, g, part, parts) : grad_sumsq<GN_MANY>(stream, g, part, parts);
 }
 
-int grad_scale(cudaStream_t stream, int count, const void* const* grads, void* const* outs, const long long* sizes,
-               const int* types, const int* out_types, int zero, double max_norm, double eps, const double* stats,
+// Every tensor times its coefficient, and the results, from the partial sums.
+template <int N>
+int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2* part, double max_norm, double eps,
                float* norm, long long* bad) {
-  GradTable t;
-  if (outs)
-    for (int i0 = 0; i0 < count; i0 += GN_TENSORS) {
-      const int blocks = fill_table(t, i0, count, grads, outs, sizes, types, out_types);
-      if (blocks < 0) return cudaErrorInvalidValue;
-      if (blocks) k_grad_scale<<<blocks, GN_THREADS, 0, stream>>>(t, stats, max_norm, eps, zero);
+  GradTable<N> t;
+  bool first = true;
+  for (int i0 = 0; g.out && i0 < g.count; i0 += N) {
+    const int blocks = fill_table(t, i0, g.count, g.in, g.out, g.sizes, g.types, g.out_types);
+    if (blocks < 0) return cudaErrorInvalidValue;
+    if (!blocks) continue;
+    int e = 0;
+    if (first) {
+      e = launch_after(stream, blocks, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero, norm, bad);
+    } else {  // (a launch that waits for a waiting one would not wait for the sums)
+      k_grad_scale<N><<<blocks, GN_THREADS, 0, stream>>>(t, parts, part, max_norm, eps, g.zero, nullptr, nullptr);
+      e = (int)cudaGetLastError();
     }
-  if (norm || bad) k_grad_result<<<1, 1, 0, stream>>>(stats, norm, bad);
-  return (int)cudaGetLastError();
+    if (e) return e;
+    first = false;
+  }
+  if (!first || (!norm && !bad)) return 0;
+  return launch_after(stream, 1, k_grad_finish, parts, part, nullptr, norm, bad);
 }
+int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2* part, double max_norm, double eps,
+               float* norm, long long* bad) {
+  return g.count <= GN_FEW ? grad_scale<GN_FEW>(stream, g, parts, part, max_norm, eps, norm, bad)
+                           : grad_scale<GN_MANY>(stream, g, parts, part, max_norm, eps, norm, bad);
+}
+
+bool limits_ok(double max_norm, double eps) { return max_norm >= 0 && eps >= 0 && std::isfinite(eps); }
 
 }  // namespace
 
@@ -151,44 +209,50 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
 
 long long nb_g1_grad_work_bytes(int count) {
   if (count < 0) return -1;
-  return 16ll + 16ll * GN_MAX_BLOCKS * grad_launches(count);
+  return 16ll * GN_BLOCKS * std::max(1, grad_launches(count));
 }
 
 int nb_g1_grad_sumsq(cudaStream_t stream, int count, const void* const* grads, const long long* sizes,
                      const int* types, int zero_nonfinite, void* work, double* stats) {
-  if (!grads_ok(count, grads, sizes, types) || !work || !stats) return (int)cudaErrorInvalidValue;
-  return grad_sumsq(stream, count, grads, sizes, types, zero_nonfinite, static_cast<double*>(work) + 2, stats);
+  if (!grads_ok(count, grads, sizes, types) || !work || !stats || reinterpret_cast<uintptr_t>(work) % 16 ||
+      reinterpret_cast<uintptr_t>(stats) % 16)
+    return (int)cudaErrorInvalidValue;
+  double2* part = static_cast<double2*>(work);
+  int parts = 0;
+  const int e = grad_sumsq(stream, {count, grads, nullptr, sizes, types, nullptr, zero_nonfinite}, part, &parts);
+  if (e) return e;
+  return launch_after(stream, 1, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr, nullptr);
 }
 
 int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
                      const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
                      double max_norm, double eps, const double* stats, float* norm, long long* bad) {
-  if (!grads_ok(count, grads, sizes, types) || !stats || std::isnan(max_norm) || max_norm < 0 || std::isnan(eps) ||
-      eps < 0)
+  if (!grads_ok(count, grads, sizes, types) || !stats || reinterpret_cast<uintptr_t>(stats) % 16 ||
+      !limits_ok(max_norm, eps))
     return (int)cudaErrorInvalidValue;
   if (outs) {
     const int e = outs_error(count, grads, outs, sizes, types, out_types);
     if (e) return e;
   }
-  return grad_scale(stream, count, grads, outs, sizes, types, out_types, zero_nonfinite, max_norm, eps, stats, norm,
-                    bad);
+  return grad_scale(stream, {count, grads, outs, sizes, types, out_types, zero_nonfinite}, 1,
+                    reinterpret_cast<const double2*>(stats), max_norm, eps, norm, bad);
 }
 
 int nb_g1_grad_clip(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
                     const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
                     double max_norm, double eps, void* work, float* norm, long long* bad) {
-  if (!grads_ok(count, grads, sizes, types) || !work || std::isnan(max_norm) || max_norm < 0 || std::isnan(eps) ||
-      eps < 0)
+  if (!grads_ok(count, grads, sizes, types) || !work || reinterpret_cast<uintptr_t>(work) % 16 ||
+      !limits_ok(max_norm, eps))
     return (int)cudaErrorInvalidValue;
   if (outs) {
     const int e = outs_error(count, grads, outs, sizes, types, out_types);
     if (e) return e;
   }
-  double* stats = static_cast<double*>(work);
-  const int e = grad_sumsq(stream, count, grads, sizes, types, zero_nonfinite, stats + 2, stats);
-  if (e) return e;
-  return grad_scale(stream, count, grads, outs, sizes, types, out_types, zero_nonfinite, max_norm, eps, stats, norm,
-                    bad);
+  const GradList g = {count, grads, outs, sizes, types, out_types, zero_nonfinite};
+  double2* part = static_cast<double2*>(work);
+  int parts = 0;
+  const int e = grad_sumsq(stream, g, part, &parts);
+  return e ? e : grad_scale(stream, g, parts, part, max_norm, eps, norm, bad);
 }
 
 }  // extern "C"
