@@ -1,4 +1,5 @@
-"""Build the CUDA library libnabla_g1.so for sm_100a, in-tree (nablaengine_b200/lib/).
+"""Build the CUDA library libnabla_g1.so for sm_100a and its torch host module nb_torch.so, in-tree
+(nablaengine_b200/lib/).
 
 nvcc cross-compiles without a GPU, so this runs anywhere the CUDA toolkit is installed; the built .so travels with
 the repository to the GPU machines. `python -m nablaengine_b200.build` rebuilds when a source is newer than the
@@ -8,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -48,6 +50,42 @@ def stale(lib=LIB, extra=()):
     return not stamp.exists() or stamp.read_text() != _flags_text(extra)
 
 
+TORCH_LIB = LIBDIR / "nb_torch.so"
+TORCH_DEPS = [CSRC / "nb_torch.cpp", PKG.parent / "include" / "nabla_g1.h"]
+
+
+def _torch_command(out):
+    """The host compiler's command for nb_torch.so (torch's and Python's headers, libnabla_g1.so beside it)."""
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+               sysconfig.get_paths()["include"], cuda]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include],
+            str(TORCH_DEPS[0]), "-o", str(out), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch_cuda", "-ltorch_python", f"-L{LIBDIR}", "-lnabla_g1", "-Wl,-rpath,$ORIGIN",
+            f"-Wl,-rpath,{root / 'lib'}"], torch.__version__
+
+
+def build_torch(force=False):
+    """Compile nb_torch.so (the host side of the training operators) when it is missing, older than its sources or
+    built for another torch; returns its path. libnabla_g1.so has to be there."""
+    tmp = TORCH_LIB.with_suffix(f".tmp{os.getpid()}.so")
+    cmd, version = _torch_command(tmp)
+    text = " ".join([version, *cmd[:-1]]).replace(str(tmp), "")
+    stamp = _stamp(TORCH_LIB)
+    if (not force and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == text
+            and all(p.stat().st_mtime <= TORCH_LIB.stat().st_mtime for p in TORCH_DEPS)):
+        return TORCH_LIB
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        raise RuntimeError(f"{cmd[0]} failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    stamp.write_text(text)
+    return TORCH_LIB
+
+
 PROFILE_LIB = LIBDIR / "libnabla_g1_prof.so"
 
 
@@ -76,3 +114,4 @@ def build(force=False, verbose=False, extra=(), out=None):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_torch(force="--force" in sys.argv))

@@ -22,6 +22,7 @@ NQ, NV, NU, NBODY, MAXCON, NEFC = 36, 35, 29, 31, 64, 192
 
 _LOCK = threading.Lock()
 _LIB = []
+_TORCH = []
 
 
 def declared_symbols():
@@ -94,6 +95,25 @@ def load(path=None, build_if_missing=True):
             raise RuntimeError(f"{lib_path}: compiled sizes {list(sizes)} do not match {want} / ABI {ABI_VERSION}")
         _LIB.append(lib)
         return lib
+
+
+def load_torch(build_if_missing=True):
+    """The loaded torch host module nb_torch (the training operators' checks, outputs and calls); builds it first when
+    it is missing and a compiler exists."""
+    load(build_if_missing=build_if_missing)  # (nb_torch is linked against it)
+    with _LOCK:
+        if not _TORCH:
+            import importlib.util
+            import torch  # noqa: F401  (its libraries have to be there)
+            if not _build.TORCH_LIB.exists():
+                if not build_if_missing:
+                    raise RuntimeError(f"{_build.TORCH_LIB} is missing: run `python -m nablaengine_b200.build`")
+                _build.build_torch()
+            spec = importlib.util.spec_from_file_location("nb_torch", _build.TORCH_LIB)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _TORCH.append(module)
+        return _TORCH[0]
 
 
 def sizes():

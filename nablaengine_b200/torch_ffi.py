@@ -223,9 +223,8 @@ def init(device=None):
     return {"library": str(capi._build.LIB), "nq": NQ, "nv": NV, "nu": NU, "nbody": NBODY, "maxcon": MAXCON}
 
 
-def _launch(dev, entry, *args, refused=None):
-    """Call the library entry on torch's current stream of device dev; a nonzero CUDA error raises (with `refused`, an
-    argument the entry refuses raises ValueError with that text)."""
+def _launch(dev, entry, *args):
+    """Call the library entry on torch's current stream of device dev; a nonzero CUDA error raises."""
     import torch
     lib = capi.load()
     stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
@@ -235,8 +234,6 @@ def _launch(dev, entry, *args, refused=None):
         with torch.cuda.device(dev):
             rc = getattr(lib, entry)(stream, *args)
     if rc:
-        if rc == 1 and refused is not None:  # cudaErrorInvalidValue, before any launch
-            raise _fail(refused, ValueError)
         raise _fail(f"{entry} failed (CUDA error {rc})", RuntimeError)
 
 
@@ -347,171 +344,41 @@ def jacobian(tape, friction, com, *, substeps=SUBSTEPS, clamp_kv=1, normal=0, ct
 # ---- the training operators: layer norm, the global gradient norm and clipping ------------------------------------
 LAYER_NORM_EPS, CLIP_EPS = 1e-5, 1e-6
 NONFINITE_MODES = ("keep", "zero")
-_OVERLAP = "a clipped gradient may not share memory with another gradient or output (but may be its own gradient)"
-_CODES = {}
+_NATIVE = []
 
 
-def _codes():
-    """{torch dtype: the C entries' type code} of the value types."""
-    if not _CODES:
-        import torch
-        _CODES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    return _CODES
+def _native():
+    """The compiled host module: it checks the arguments (TypeError, ValueError), makes the outputs and launches on
+    torch's current stream of the tensors' device."""
+    if not _NATIVE:
+        _NATIVE.append(capi.load_torch())
+    return _NATIVE[0]
 
 
-def _norm_rows(name, x):
-    """(rows, row stride) of a layer norm argument: a CUDA tensor of a value type with at least one dimension and one
-    column, its last dimension dense and its leading dimensions one uniform stride apart (a column slice of a wider
-    buffer passes, a transposed tensor does not)."""
+def _tensor_list(name, x):
     import torch
-    ok = isinstance(x, torch.Tensor) and x.dtype in _codes() and x.is_cuda and x.dim() >= 1 and x.shape[-1] >= 1
-    if ok:
-        cols = x.shape[-1]
-        rows = x.numel() // cols
-        if x.is_contiguous():
-            return rows, cols
-        if cols == 1 or x.stride(-1) == 1:
-            lead = [(n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
-            if rows == 0 or all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:])):
-                return rows, lead[-1][1] if lead and rows else cols
-    raise _fail(f"{name} must be a float32, bfloat16 or float16 CUDA tensor (..., columns) with dense columns and "
-                f"rows one stride apart, got {_describe(x)}")
-
-
-def _norm_param(name, p, x):
-    """Check a layer norm parameter: None, or a contiguous (columns,) tensor of x's type or float32 on x's device."""
-    import torch
-    if p is None:
-        return
-    if not (isinstance(p, torch.Tensor) and (p.dtype == x.dtype or p.dtype == torch.float32) and p.dim() == 1
-            and p.shape[0] == x.shape[-1] and p.is_contiguous() and p.device == x.device):
-        raise _fail(f"{name} must be a contiguous ({x.shape[-1]},) tensor of x's type or float32 on {x.device}, got "
-                    f"{_describe(p)}")
-
-
-def _norm_params(weight, bias, x):
-    """Check weight and bias against x; returns their type code (x's own if there are none)."""
-    _norm_param("weight", weight, x)
-    _norm_param("bias", bias, x)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise _fail(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    p = weight if weight is not None else bias if bias is not None else x
-    return _codes()[p.dtype]
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _layer_norm_impl(x, weight, bias, eps):
-    import torch
-    rows, stride = _norm_rows("x", x)
-    wcode = _norm_params(weight, bias, x)
-    e = float(eps)
-    if not (math.isfinite(e) and e >= 0.0):
-        raise _fail(f"eps must be finite and >= 0, got {eps}", ValueError)
-    dev = x.get_device()
-    _device(dev)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    if rows:
-        _launch(dev, "nb_g1_layer_norm_forward", rows, x.shape[-1], stride, _codes()[x.dtype], x.data_ptr(), wcode,
-                _ptr(weight), _ptr(bias), e, y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
-    return y, mean, rstd
-
-
-def _layer_norm_backward_impl(g_y, x, mean, rstd, weight, bias, want_x=True, want_weight=True, want_bias=True):
-    import torch
-    rows, stride = _norm_rows("x", x)
-    grows, gstride = _norm_rows("g_y", g_y)
-    wcode = _norm_params(weight, bias, x)
-    if g_y.shape != x.shape or g_y.dtype != x.dtype or g_y.device != x.device:
-        raise _fail(f"g_y must be like x ({_describe(x)}), got {_describe(g_y)}")
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        if not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.shape == x.shape[:-1]
-                and t.is_contiguous() and t.device == x.device):
-            raise _fail(f"{name} must be a contiguous torch.float32 tensor of shape {tuple(x.shape[:-1])} on "
-                        f"{x.device}, got {_describe(t)}")
-    dev, cols = x.get_device(), x.shape[-1]
-    _device(dev)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-    gw = torch.empty_like(weight) if want_weight and weight is not None else None
-    gb = torch.empty_like(bias) if want_bias and bias is not None else None
-    work = None
-    if gw is not None or gb is not None:
-        nwork = int(capi.load().nb_g1_layer_norm_work_bytes(rows, cols))
-        work = torch.empty((nwork,), dtype=torch.uint8, device=x.device)
-    if rows or work is not None:
-        _launch(dev, "nb_g1_layer_norm_backward", rows, cols, gstride, stride, _codes()[x.dtype], g_y.data_ptr(),
-                x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), wcode, _ptr(weight), _ptr(gx), _ptr(gw), _ptr(gb),
-                _ptr(work))
-    return gx, gw, gb
-
-
-def _dense(t):
-    """True when t's values fill one span of memory, in any order of its dimensions."""
-    if t.is_contiguous():
-        return True
-    span = 1
-    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
-        if s != span:
-            return False
-        span *= n
-    return True
-
-
-def _grad_list(name, grads):
-    """Check a gradient list: dense CUDA tensors of the value types on one device; returns it as a list."""
-    import torch
-    if isinstance(grads, torch.Tensor):  # (its rows would be taken one by one)
+    if isinstance(x, (list, tuple)):
+        return x
+    if isinstance(x, torch.Tensor):  # (its rows would be taken one by one)
         raise _fail(f"{name} must be a list of tensors, got one tensor")
-    grads, codes = list(grads), _codes()
-    for i, g in enumerate(grads):
-        if not (isinstance(g, torch.Tensor) and g.dtype in codes and g.is_cuda and _dense(g)):
-            raise _fail(f"{name}[{i}] must be a dense float32, bfloat16 or float16 CUDA tensor, got {_describe(g)}")
-        if g.get_device() != grads[0].get_device():
-            raise _fail(f"{name}[{i}] is on {g.device}, {name}[0] on {grads[0].device}")
-    return grads
-
-
-def _host_arrays(grads):
-    """The ctypes arrays of a gradient list: addresses, value counts, type codes."""
-    n, codes = len(grads), _codes()
-    return ((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]),
-            (ctypes.c_longlong * n)(*[g.numel() for g in grads]), (ctypes.c_int * n)(*[codes[g.dtype] for g in grads]))
+    return list(x)
 
 
 def _zero_mode(nonfinite):
     if nonfinite not in NONFINITE_MODES:
         raise _fail(f"nonfinite must be one of {NONFINITE_MODES}, got {nonfinite!r}", ValueError)
-    return 1 if nonfinite == "zero" else 0
+    return nonfinite == "zero"
 
 
 def _clip_impl(grads, outs, max_norm, eps, zero, group):
-    """The norm of checked gradients, and, with outs, the clipped gradients: (norm, bad)."""
-    import torch
-    at = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
-    dev = at.index
-    _device(dev)
-    addr, sizes, types = _host_arrays(grads)
-    out_addr, out_types = None, None
-    if outs is not None:
-        out_addr, _, out_types = _host_arrays(outs)
-    norm = torch.empty((), dtype=torch.float32, device=at)
-    bad = torch.empty((), dtype=torch.int64, device=at)
-    work = torch.empty((int(capi.load().nb_g1_grad_work_bytes(len(grads))),), dtype=torch.uint8, device=at)
-    if group is None:
-        _launch(dev, "nb_g1_grad_clip", len(grads), addr, out_addr, sizes, types, out_types, zero, max_norm, eps,
-                work.data_ptr(), norm.data_ptr(), bad.data_ptr(), refused=_OVERLAP)
-        return norm, bad
-    import torch.distributed as dist
-    stats = torch.empty((2,), dtype=torch.float64, device=at)
-    _launch(dev, "nb_g1_grad_sumsq", len(grads), addr, sizes, types, zero, work.data_ptr(), stats.data_ptr())
-    dist.all_reduce(stats, op=dist.ReduceOp.SUM, group=group)
-    _launch(dev, "nb_g1_grad_scale", len(grads), addr, out_addr, sizes, types, out_types, zero, max_norm, eps,
-            stats.data_ptr(), norm.data_ptr(), bad.data_ptr(), refused=_OVERLAP)
-    return norm, bad
+    """The norm of the gradients and, with outs, the clipped gradients: (norm, bad). With a group, the sums of its
+    ranks are added up between the two passes."""
+    native, stats = _native(), None
+    if group is not None:
+        import torch.distributed as dist
+        stats, = native.grad_sumsq(grads, zero)
+        dist.all_reduce(stats, op=dist.ReduceOp.SUM, group=group)
+    return native.grad_clip(grads, outs, max_norm, eps, zero, stats)
 
 
 # ---- custom ops (torch.library): the library calls as opaque graph nodes, traced by torch.compile ---------------
@@ -569,7 +436,7 @@ def _register_ops():
 
     @torch.library.custom_op("nabla_b200::layer_norm", mutates_args=())
     def layer_norm_op(x: T, weight: Optional[T], bias: Optional[T], eps: float) -> List[T]:
-        return list(_layer_norm_impl(x, weight, bias, eps))
+        return list(_native().layer_norm(x, weight, bias, eps))
 
     @layer_norm_op.register_fake
     def _(x, weight, bias, eps):
@@ -578,7 +445,7 @@ def _register_ops():
     @torch.library.custom_op("nabla_b200::layer_norm_backward", mutates_args=())
     def layer_norm_backward_op(g_y: T, x: T, mean: T, rstd: T, weight: Optional[T], bias: Optional[T], want_x: bool,
                                want_weight: bool, want_bias: bool) -> List[T]:
-        r = _layer_norm_backward_impl(g_y, x, mean, rstd, weight, bias, want_x, want_weight, want_bias)
+        r = _native().layer_norm_backward(g_y, x, mean, rstd, weight, bias, want_x, want_weight, want_bias)
         return [x.new_empty((0,)) if t is None else t for t in r]
 
     @layer_norm_backward_op.register_fake
@@ -665,7 +532,7 @@ def _autograd_function(name):
             if _tracing():
                 y, mean, rstd = custom_ops()["layer_norm"](x, weight, bias, eps)
             else:
-                y, mean, rstd = _layer_norm_impl(x, weight, bias, eps)
+                y, mean, rstd = _native().layer_norm(x, weight, bias, eps)
             ctx.save_for_backward(x, mean, rstd, weight, bias)
             return y
 
@@ -678,7 +545,7 @@ def _autograd_function(name):
             if _tracing():
                 r = custom_ops()["layer_norm_backward"](g_y, x, mean, rstd, weight, bias, *want)
             else:
-                r = _layer_norm_backward_impl(g_y, x, mean, rstd, weight, bias, *want)
+                r = _native().layer_norm_backward(g_y, x, mean, rstd, weight, bias, *want)
             return tuple(g if w else None for g, w in zip(r, want)) + (None,)
 
     class GradScale(torch.autograd.Function):
@@ -813,8 +680,9 @@ def layer_norm(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
 def layer_norm_forward(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
     """layer_norm without autograd: (y, mean, rstd), the rows' statistics in float32 with x's leading dimensions, which
     layer_norm_backward takes."""
-    args = (x, weight, bias, float(eps))
-    return tuple(custom_ops()["layer_norm"](*args)) if _tracing() else _layer_norm_impl(*args)
+    if _tracing():
+        return tuple(custom_ops()["layer_norm"](x, weight, bias, float(eps)))
+    return _native().layer_norm(x, weight, bias, eps)
 
 
 def layer_norm_backward(g_y, x, mean, rstd, weight=None, bias=None):
@@ -824,7 +692,7 @@ def layer_norm_backward(g_y, x, mean, rstd, weight=None, bias=None):
     if _tracing():
         gx, gw, gb = custom_ops()["layer_norm_backward"](g_y, x, mean, rstd, weight, bias, True, True, True)
         return gx, None if weight is None else gw, None if bias is None else gb
-    return _layer_norm_backward_impl(g_y, x, mean, rstd, weight, bias)
+    return _native().layer_norm_backward(g_y, x, mean, rstd, weight, bias, True, True, True)
 
 
 def grad_norm(grads, *, nonfinite="keep", group=None):
@@ -832,8 +700,7 @@ def grad_norm(grads, *, nonfinite="keep", group=None):
     copied to the host): the root of the sum of all squares, summed in 64 bits, and the number of non-finite values.
     nonfinite: "keep" (they take part, the norm is infinite or NaN) or "zero" (they count as 0). group: a
     torch.distributed process group whose ranks each hold a part of the gradient (the sums are added up over it)."""
-    grads = _grad_list("grads", grads)
-    return _clip_impl(grads, None, 0.0, 0.0, _zero_mode(nonfinite), group)
+    return _clip_impl(_tensor_list("grads", grads), None, 0.0, 0.0, _zero_mode(nonfinite), group)
 
 
 def clip_grad_norm(grads, max_norm, *, eps=CLIP_EPS, nonfinite="keep", out=None, group=None):
@@ -843,25 +710,9 @@ def clip_grad_norm(grads, max_norm, *, eps=CLIP_EPS, nonfinite="keep", out=None,
     non-finite values become 0 and the others are clipped by the norm without them. grads: dense CUDA tensors
     (float32, bfloat16, float16, mixed) on one device, no two overlapping. Under torch.no_grad semantics: nothing is
     differentiated through."""
-    import torch
-    limit, e, zero = float(max_norm), float(eps), _zero_mode(nonfinite)
-    if not limit >= 0.0 or not (math.isfinite(e) and e >= 0.0):
-        raise _fail(f"max_norm and eps must be >= 0 (eps finite), got {max_norm}, {eps}", ValueError)
-    grads = _grad_list("grads", grads)
-    outs = grads if out is None else _grad_list("out", out)
-    if out is not None:
-        if len(outs) != len(grads):
-            raise _fail(f"out must have as many tensors as grads ({len(grads)}), got {len(outs)}")
-        for i, (o, g) in enumerate(zip(outs, grads)):
-            if (o.shape != g.shape or o.device != g.device or (o.dtype != g.dtype and o.dtype != torch.float32)
-                    or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
-                raise _fail(f"out[{i}] must be like grads[{i}] ({_describe(g)}) or its float32 form, got "
-                            f"{_describe(o)}")
-    try:
-        norm, bad = _clip_impl(grads, outs, limit, e, zero, group)
-    finally:
-        torch.autograd.graph.increment_version(outs)
-    return norm, bad
+    grads = _tensor_list("grads", grads)
+    outs = grads if out is None else _tensor_list("out", out)
+    return _clip_impl(grads, outs, max_norm, eps, _zero_mode(nonfinite), group)
 
 
 # ---- diagnostics -------------------------------------------------------------------------------------------------

@@ -94,49 +94,27 @@ def test_torch_api_refuses_cpu_tensors():
             call()
 
 
-def test_dense_layouts():
-    t = torch.zeros(4, 6, 5)
-    for dense in (t, t.permute(2, 0, 1), t[:1], t[:, :, :1].contiguous(), t.new_zeros(0, 3), t.new_zeros(())):
-        assert torch_ffi._dense(dense)
-    for gaps in (t[:, :, ::2], t[:, 1:], t[:, :, :1], t[0, 0].expand(3, 5)):
-        assert not torch_ffi._dense(gaps)
+class _StandIn:
+    """The compiled host module's two calls on CPU tensors."""
 
+    @staticmethod
+    def grad_sumsq(grads, zero):
+        s = sum(float((g.double() ** 2).sum()) for g in grads)
+        return torch.tensor([s, 0.0], dtype=torch.float64),
 
-def _stand_in(monkeypatched):
-    """The device calls on CPU tensors: sums of squares and scaling by the two sums, through the addresses given."""
-    import numpy as np
-
-    def values(addr, n):
-        return np.ctypeslib.as_array((ctypes.c_float * n).from_address(addr))
-
-    def launch(dev, entry, count, addr, *rest, refused=None):
-        if entry == "nb_g1_grad_sumsq":
-            sizes, _, zero, _, stats = rest
-            vals = [values(addr[i], sizes[i]) for i in range(count)]
-            out = np.ctypeslib.as_array((ctypes.c_double * 2).from_address(stats))
-            out[0] = sum(float((v.astype(np.float64) ** 2).sum()) for v in vals)
-            out[1] = 0.0
-        elif entry == "nb_g1_grad_scale":
-            outs, sizes, _, _, zero, max_norm, eps, stats, norm, bad = rest
-            s = np.ctypeslib.as_array((ctypes.c_double * 2).from_address(stats))
-            n = float(s[0]) ** 0.5
-            (ctypes.c_float).from_address(norm).value = n
-            (ctypes.c_longlong).from_address(bad).value = int(s[1])
-            for i in range(count if outs else 0):
-                values(outs[i], sizes[i])[:] = values(addr[i], sizes[i]) * min(1.0, max_norm / (n + eps))
-        else:
-            raise AssertionError(entry)
-
-    monkeypatched("_launch", launch)
-    monkeypatched("_device", lambda dev: None)
-    monkeypatched("_grad_list", lambda name, grads: list(grads))
+    @staticmethod
+    def grad_clip(grads, outs, max_norm, eps, zero, stats):
+        norm = float(stats[0]) ** 0.5
+        for o, g in zip(outs or (), grads):
+            o.copy_(g * min(1.0, max_norm / (norm + eps)))
+        return torch.tensor(norm), stats[1].long()
 
 
 def _rank_main(rank, world, port, out):
     import torch.distributed as dist
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
     dist.init_process_group("gloo", rank=rank, world_size=world)
-    _stand_in(lambda name, value: setattr(torch_ffi, name, value))
+    torch_ffi._NATIVE[:] = [_StandIn]
     g = torch.Generator().manual_seed(5)
     full = torch.randn(2, 1000, generator=g)
     mine = [full[rank].clone()]
