@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
   __shared__ float2 slots[64];
   constexpr int THREADS = ln_threads(LANES, sizeof(T), true), GROUPS = THREADS / LANES, N2 = EPT / 2;
   const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the sum of the parts may be set up meanwhile)
   LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
   const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;
   const float inv = 1.f / cols;
@@ -396,27 +397,30 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
   }
 }
 
-// gw, gb = the sums of the blocks' column sums: 32 columns a block, 8 threads to a column
+// gw, gb = the sums of the blocks' column sums: 32 columns a block, a warp for each 32nd of the parts
 template <class W>
-__global__ void __launch_bounds__(256) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
-                                                         W* __restrict__ gw, W* __restrict__ gb) {
-  __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
+                                                          W* __restrict__ gw, W* __restrict__ gb) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;  // 0 .. 2 cols: gw's columns, then gb's
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float v = 0.f;
   if (c < 2 * cols) {
 #pragma unroll 8
-    for (int p = warp; p < parts; p += 8) v += part[(long long)p * 2 * cols + c];
+    for (int p = warp; p < parts; p += 32) v += part[(long long)p * 2 * cols + c];
   }
   s[warp][lane] = v;
   __syncthreads();
-  if (warp || c >= 2 * cols) return;
+  v = s[lane][warp];  // (a warp per column now)
 #pragma unroll
-  for (int k = 1; k < 8; k++) v += s[k][lane];
-  if (c < cols) {
-    if (gw) gw[c] = from_f32<W>(v);
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  const int mine = blockIdx.x * 32 + warp;
+  if (lane || mine >= 2 * cols) return;
+  if (mine < cols) {
+    if (gw) gw[mine] = from_f32<W>(v);
   } else if (gb) {
-    gb[c - cols] = from_f32<W>(v);
+    gb[mine - cols] = from_f32<W>(v);
   }
 }
 

@@ -5,6 +5,7 @@
 #include <cstdint>
 #include <type_traits>
 #include "nb_layer_norm.cuh"
+#include "nb_launch.h"
 #include "nb_layer_norm_call.h"
 
 namespace nbtrain {
@@ -175,10 +176,10 @@ template <class T> int ln_backward(const LnBackward& a) {
   if (e || !sums) return e;
   ln_param_type<T>(a.wtype, [&](auto w) {
     using W = decltype(w);
-    k_ln_backward_sum<W><<<(2 * a.cols + 31) / 32, 256, 0, a.stream>>>(parts, a.cols, a.part, static_cast<W*>(a.gw),
-                                                                       static_cast<W*>(a.gb));
+    e = launch_after(a.stream, (2 * a.cols + 31) / 32, 1024, k_ln_backward_sum<W>, parts, a.cols, a.part,
+                     static_cast<W*>(a.gw), static_cast<W*>(a.gb));
   });
-  return (int)cudaGetLastError();
+  return e;
 }
 
 }  // namespace nbtrain

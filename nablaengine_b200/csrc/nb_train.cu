@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <new>
 #include "nb_grad_norm.cuh"
+#include "nb_launch.h"
 #include "nb_layer_norm_call.h"
 
 using namespace nbtrain;
@@ -98,21 +99,6 @@ int fill_table(GradTable<N>& t, int i0, int count, const void* const* in, void* 
   return (int)std::min<long long>(chunks, GN_BLOCKS);
 }
 
-// Launch a kernel that may start while the one before it in the stream ends (it waits for it before its first access).
-template <class... P, class... A>
-int launch_after(cudaStream_t stream, int blocks, void (*kernel)(P...), A... args) {
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(blocks);
-  config.blockDim = dim3(GN_THREADS);
-  config.stream = stream;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
-}
-
 struct GradList {
   int count;
   const void* const* in;
@@ -151,7 +137,7 @@ int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2*
     if (!blocks) continue;
     int e = 0;
     if (first) {
-      e = launch_after(stream, blocks, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero, norm, bad);
+      e = launch_after(stream, blocks, GN_THREADS, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero, norm, bad);
     } else {  // (a launch that waits for a waiting one would not wait for the sums)
       k_grad_scale<N><<<blocks, GN_THREADS, 0, stream>>>(t, parts, part, max_norm, eps, g.zero, nullptr, nullptr);
       e = (int)cudaGetLastError();
@@ -160,7 +146,7 @@ int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2*
     first = false;
   }
   if (!first || (!norm && !bad)) return 0;
-  return launch_after(stream, 1, k_grad_finish, parts, part, nullptr, norm, bad);
+  return launch_after(stream, 1, GN_THREADS, k_grad_finish, parts, part, nullptr, norm, bad);
 }
 int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2* part, double max_norm, double eps,
                float* norm, long long* bad) {
@@ -221,7 +207,7 @@ int nb_g1_grad_sumsq(cudaStream_t stream, int count, const void* const* grads, c
   int parts = 0;
   const int e = grad_sumsq(stream, {count, grads, nullptr, sizes, types, nullptr, zero_nonfinite}, part, &parts);
   if (e) return e;
-  return launch_after(stream, 1, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr, nullptr);
+  return launch_after(stream, 1, GN_THREADS, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr, nullptr);
 }
 
 int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
