@@ -243,7 +243,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_grad_scale(const __grid_constant
   const float coef = clip_coefficient(stats.x, max_norm, eps);
   const bool clean = zero && stats.y > 0.0;
   int i = t.count - 1;
-  for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+  // (the chunks that this block had in the first pass, back from the last one)
+  for (int c = blockIdx.x + (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x; c >= (int)blockIdx.x;
+       c -= gridDim.x) {
     while (t.t[i].first > c) i--;
     const GradEntry& e = t.t[i];
     if (coef == 1.f && !clean && e.in == e.out) continue;  // (in place, and every value stays as it is)

@@ -366,61 +366,53 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
     }
   }
   if (!part) return;
-  // the groups' column sums: over the groups of a warp by shuffles, then group by group through shared memory
+  // the column sums of the block: of its one group, or of its groups, (GROUPS, 2, cols) over the ring
+  float* sums = part + (long long)blockIdx.x * 2 * cols;
+  float* mine = GROUPS == 1 ? sums : reinterpret_cast<float*>(ring) + g.index * 2 * cols;
+  if (GROUPS > 1) {
+    copy_wait(0);
+    __syncthreads();
+  }
 #pragma unroll
-  for (int m = LANES; m < 32; m <<= 1) {
-#pragma unroll
-    for (int i = 0; i < N2; i++) {
-      gw[i].x += __shfl_xor_sync(0xffffffffu, gw[i].x, m);
-      gw[i].y += __shfl_xor_sync(0xffffffffu, gw[i].y, m);
-      gb[i].x += __shfl_xor_sync(0xffffffffu, gb[i].x, m);
-      gb[i].y += __shfl_xor_sync(0xffffffffu, gb[i].y, m);
+  for (int i = 0; i < EPT; i++) {
+    const int c = ln_column<LANES, V>(lane, i);
+    if (FULL || c < cols) {
+      mine[c] = i % 2 ? gw[i / 2].y : gw[i / 2].x;
+      mine[cols + c] = i % 2 ? gb[i / 2].y : gb[i / 2].x;
     }
   }
-  float* total = reinterpret_cast<float*>(ring);  // (2, cols), over the ring
-  constexpr int UNIT = LANES < 32 ? 32 : LANES, UNITS = THREADS / UNIT;
-  const int mine = threadIdx.x / UNIT;
-  float* sums = part + (long long)blockIdx.x * 2 * cols;
-  copy_wait(0);
-  for (int u = 0; u < UNITS; u++) {
-    __syncthreads();
-    if (u != mine || (LANES < 32 && (threadIdx.x & 31) >= LANES)) continue;
-#pragma unroll
-    for (int i = 0; i < EPT; i++) {
-      const int c = ln_column<LANES, V>(lane, i);
-      if (c >= cols) continue;
-      float a = i % 2 ? gw[i / 2].y : gw[i / 2].x, d = i % 2 ? gb[i / 2].y : gb[i / 2].x;
-      if (u) a += total[c], d += total[cols + c];
-      if (u + 1 < UNITS) total[c] = a, total[cols + c] = d;
-      else sums[c] = a, sums[cols + c] = d;
-    }
+  if (GROUPS == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * cols; c += THREADS) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < GROUPS; k++) v += reinterpret_cast<const float*>(ring)[k * 2 * cols + c];
+    sums[c] = v;
   }
 }
 
-// gw, gb = the sums of the blocks' column sums: 32 columns a block, a warp for each 32nd of the parts
-template <class W>
-__global__ void __launch_bounds__(1024) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
-                                                          W* __restrict__ gw, W* __restrict__ gb) {
-  __shared__ float s[32][33];
+// gw, gb = the sums of the blocks' column sums: 32 columns a block, a warp for each WARPS-th of the parts
+template <class W, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
+                                                                W* __restrict__ gw, W* __restrict__ gb) {
+  __shared__ float s[WARPS][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;  // 0 .. 2 cols: gw's columns, then gb's
   asm volatile("griddepcontrol.wait;" ::: "memory");
   float v = 0.f;
   if (c < 2 * cols) {
-#pragma unroll 8
-    for (int p = warp; p < parts; p += 32) v += part[(long long)p * 2 * cols + c];
+#pragma unroll 10
+    for (int p = warp; p < parts; p += WARPS) v += part[(long long)p * 2 * cols + c];
   }
   s[warp][lane] = v;
   __syncthreads();
-  v = s[lane][warp];  // (a warp per column now)
+  if (warp || c >= 2 * cols) return;
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-  const int mine = blockIdx.x * 32 + warp;
-  if (lane || mine >= 2 * cols) return;
-  if (mine < cols) {
-    if (gw) gw[mine] = from_f32<W>(v);
+  for (int k = 1; k < WARPS; k++) v += s[k][lane];
+  if (c < cols) {
+    if (gw) gw[c] = from_f32<W>(v);
   } else if (gb) {
-    gb[mine - cols] = from_f32<W>(v);
+    gb[c - cols] = from_f32<W>(v);
   }
 }
 

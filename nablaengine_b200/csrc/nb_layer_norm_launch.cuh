@@ -176,8 +176,12 @@ template <class T> int ln_backward(const LnBackward& a) {
   if (e || !sums) return e;
   ln_param_type<T>(a.wtype, [&](auto w) {
     using W = decltype(w);
-    e = launch_after(a.stream, (2 * a.cols + 31) / 32, 1024, k_ln_backward_sum<W>, parts, a.cols, a.part,
-                     static_cast<W*>(a.gw), static_cast<W*>(a.gb));
+    // (many warps to a column where there are few columns, few where a block would wait for its place)
+    auto sum = [&](auto warps) {
+      return launch_after(a.stream, (2 * a.cols + 31) / 32, 32 * warps.value, k_ln_backward_sum<W, warps.value>, parts,
+                          a.cols, a.part, static_cast<W*>(a.gw), static_cast<W*>(a.gb));
+    };
+    e = a.cols <= 2048 ? sum(Int<32>()) : sum(Int<8>());
   });
   return e;
 }
