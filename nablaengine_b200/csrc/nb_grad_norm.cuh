@@ -127,7 +127,8 @@ __device__ __forceinline__ double2 block_sum(double2 v) {
 template <int N>
 __global__ void __launch_bounds__(GN_THREADS) k_grad_sumsq(const __grid_constant__ GradTable<N> t, int zero, int base,
                                                            double2* __restrict__ part) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_start();
+  wait_for_last();
   double s = 0.0, bad = 0.0;
   int i = 0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
@@ -157,7 +158,8 @@ __device__ __forceinline__ double2 sum_parts(int parts, const double2* part) {
 __global__ void __launch_bounds__(GN_THREADS) k_grad_finish(int parts, const double2* __restrict__ part,
                                                             double2* __restrict__ stats, float* __restrict__ norm,
                                                             long long* __restrict__ bad) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_next_start();
+  wait_for_last();
   const double2 v = sum_parts(parts, part);
   if (threadIdx.x) return;
   if (stats) *stats = v;
@@ -234,7 +236,8 @@ __global__ void __launch_bounds__(GN_THREADS) k_grad_scale(const __grid_constant
                                                            const double2* __restrict__ part, double max_norm,
                                                            double eps, int zero, float* __restrict__ norm,
                                                            long long* __restrict__ bad) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_next_start();
+  wait_for_last();
   const double2 stats = sum_parts(parts, part);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     if (norm) *norm = (float)sqrt(stats.x);

@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
   __shared__ float2 slots[64];
   constexpr int THREADS = ln_threads(LANES, sizeof(T), false), GROUPS = THREADS / LANES, N2 = EPT / 2;
   const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
+  let_next_start();
   LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
   const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;  // the group's place in its warp
   const float inv = 1.f / cols;
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
   const T* at = feed.next;
   T* out = y + turn.row * cols;
   const long long out_step = turn.step * cols;
+  wait_for_last();
   for (int s = 0; s + 1 < t.stages; s++) fill(s);
   float2 w[N2], b[N2];
   load_param<LANES, EPT, V>(weight, wtype, 1.f, cols, lane, w);
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
   __shared__ float2 slots[64];
   constexpr int THREADS = ln_threads(LANES, sizeof(T), true), GROUPS = THREADS / LANES, N2 = EPT / 2;
   const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the sum of the parts may be set up meanwhile)
+  let_next_start();
   LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
   const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;
   const float inv = 1.f / cols;
@@ -315,6 +317,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
   const T *xat = xfeed.next, *gat = gfeed.next;
   T* out = gx + turn.row * cols;
   const long long out_step = turn.step * cols;
+  wait_for_last();
   for (int s = 0; s + 1 < t.stages; s++) fill(s);
   float2 w[N2], gw[N2], gb[N2];
   load_param<LANES, EPT, V>(weight, wtype, 1.f, cols, lane, w);
@@ -398,7 +401,8 @@ __global__ void __launch_bounds__(32 * WARPS) k_ln_backward_sum(int parts, int c
   __shared__ float s[WARPS][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;  // 0 .. 2 cols: gw's columns, then gb's
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_next_start();
+  wait_for_last();
   float v = 0.f;
   if (c < 2 * cols) {
 #pragma unroll 10

@@ -134,9 +134,8 @@ template <class T> int ln_forward(const LnForward& a) {
     static std::atomic<bool> done[64];
     const int e = allow_smem(kernel, done);
     if (e) return e;
-    kernel<<<p.blocks, ln_threads(lanes.value, sizeof(T), false), p.smem, a.stream>>>(
-        p.t, kind, a.stride, x, a.wtype, a.weight, a.bias, a.eps, y, a.mean, a.rstd);
-    return (int)cudaGetLastError();
+    return launch_after(a.stream, p.blocks, ln_threads(lanes.value, sizeof(T), false), p.smem, kernel, p.t, kind,
+                        a.stride, x, a.wtype, a.weight, a.bias, a.eps, y, a.mean, a.rstd);
   });
 }
 
@@ -167,10 +166,9 @@ template <class T> int ln_backward(const LnBackward& a) {
       static std::atomic<bool> done[64];
       const int rc = allow_smem(kernel, done);
       if (rc) return rc;
-      kernel<<<p.blocks, ln_threads(lanes.value, sizeof(T), true), p.smem, a.stream>>>(
-          p.t, gkind, a.g_stride, kind, a.stride, g, x, a.mean, a.rstd, a.wtype, a.weight, gx,
-          sums ? a.part : nullptr);
-      return (int)cudaGetLastError();
+      return launch_after(a.stream, p.blocks, ln_threads(lanes.value, sizeof(T), true), p.smem, kernel, p.t, gkind,
+                          a.g_stride, kind, a.stride, g, x, a.mean, a.rstd, a.wtype, a.weight, gx,
+                          sums ? a.part : nullptr);
     });
   }
   if (e || !sums) return e;
@@ -178,8 +176,8 @@ template <class T> int ln_backward(const LnBackward& a) {
     using W = decltype(w);
     // (many warps to a column where there are few columns, few where a block would wait for its place)
     auto sum = [&](auto warps) {
-      return launch_after(a.stream, (2 * a.cols + 31) / 32, 32 * warps.value, k_ln_backward_sum<W, warps.value>, parts,
-                          a.cols, a.part, static_cast<W*>(a.gw), static_cast<W*>(a.gb));
+      return launch_after(a.stream, (2 * a.cols + 31) / 32, 32 * warps.value, 0, k_ln_backward_sum<W, warps.value>,
+                          parts, a.cols, a.part, static_cast<W*>(a.gw), static_cast<W*>(a.gb));
     };
     e = a.cols <= 2048 ? sum(Int<32>()) : sum(Int<8>());
   });

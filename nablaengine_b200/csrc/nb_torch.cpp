@@ -262,7 +262,7 @@ std::vector<Tensor> grad_sumsq(PyObject* const* a) {
   return {stats};
 }
 
-// (grads, outs or None, max_norm, eps, zero, stats or None) -> (norm, bad): the sums of squares are grads' own, or stats
+// (grads, outs or None, max_norm, eps, zero, stats or None) -> (norm, bad): by grads' own sums, or by stats'
 std::vector<Tensor> grad_clip(PyObject* const* a) {
   const List g = list_of("grads", a[0]);
   const double max_norm = number(a[2]), eps = number(a[3]);

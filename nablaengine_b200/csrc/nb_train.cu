@@ -116,10 +116,11 @@ template <int N> int grad_sumsq(cudaStream_t stream, const GradList& g, double2*
     const int blocks = fill_table(t, i0, g.count, g.in, nullptr, g.sizes, g.types, nullptr);
     if (blocks < 0) return cudaErrorInvalidValue;
     if (!blocks) continue;
-    k_grad_sumsq<N><<<blocks, GN_THREADS, 0, stream>>>(t, g.zero, *parts, part);
+    const int e = launch_after(stream, blocks, GN_THREADS, 0, k_grad_sumsq<N>, t, g.zero, *parts, part);
+    if (e) return e;
     *parts += blocks;
   }
-  return (int)cudaGetLastError();
+  return 0;
 }
 int grad_sumsq(cudaStream_t stream, const GradList& g, double2* part, int* parts) {
   return g.count <= GN_FEW ? grad_sumsq<GN_FEW>(stream, g, part, parts) : grad_sumsq<GN_MANY>(stream, g, part, parts);
@@ -135,18 +136,13 @@ int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2*
     const int blocks = fill_table(t, i0, g.count, g.in, g.out, g.sizes, g.types, g.out_types);
     if (blocks < 0) return cudaErrorInvalidValue;
     if (!blocks) continue;
-    int e = 0;
-    if (first) {
-      e = launch_after(stream, blocks, GN_THREADS, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero, norm, bad);
-    } else {  // (a launch that waits for a waiting one would not wait for the sums)
-      k_grad_scale<N><<<blocks, GN_THREADS, 0, stream>>>(t, parts, part, max_norm, eps, g.zero, nullptr, nullptr);
-      e = (int)cudaGetLastError();
-    }
+    const int e = launch_after(stream, blocks, GN_THREADS, 0, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero,
+                               first ? norm : nullptr, first ? bad : nullptr);
     if (e) return e;
     first = false;
   }
   if (!first || (!norm && !bad)) return 0;
-  return launch_after(stream, 1, GN_THREADS, k_grad_finish, parts, part, nullptr, norm, bad);
+  return launch_after(stream, 1, GN_THREADS, 0, k_grad_finish, parts, part, nullptr, norm, bad);
 }
 int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2* part, double max_norm, double eps,
                float* norm, long long* bad) {
@@ -207,7 +203,8 @@ int nb_g1_grad_sumsq(cudaStream_t stream, int count, const void* const* grads, c
   int parts = 0;
   const int e = grad_sumsq(stream, {count, grads, nullptr, sizes, types, nullptr, zero_nonfinite}, part, &parts);
   if (e) return e;
-  return launch_after(stream, 1, GN_THREADS, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr, nullptr);
+  return launch_after(stream, 1, GN_THREADS, 0, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr,
+                      nullptr);
 }
 
 int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, void* const* outs,

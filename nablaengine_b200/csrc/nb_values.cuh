@@ -40,6 +40,11 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
   return pair2(r);
 }
+// For kernels launched by launch_after: the next kernel may be set up from here on; and: the one before is complete and
+// its memory seen (nothing is read or written earlier).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The two values of a 32-bit word, and back.
