@@ -15,7 +15,12 @@
 
 namespace nbtrain {
 
-constexpr int LN_MAX_COLS = 16384;  // the widest row held in registers
+constexpr int LN_LANES = 256;        // lanes of a row in one block, two blocks an SM
+constexpr int LN_SPLIT_LANES = 512;  // in the backward's widest rows: one block an SM
+constexpr int LN_WIDEST = 32768;     // the widest row held in registers
+constexpr int LN_CLUSTER = 8;        // blocks of a cluster at most
+// values per lane there: 32 bytes of a row, so that four rows of both tensors fit the ring
+__host__ __device__ constexpr int ln_split_ept(int e) { return 32 / e; }
 // The threads of a block and the blocks per SM for rows of `lanes` lanes of e-byte values, as measured. Forward: one
 // large block (131072 x 512 float32 88 us, 6100 GB/s, against 97 in two of half the size; 262144 x 512 bfloat16 88
 // against 97), but two for 16-bit rows that are spread over several warps, where one computes while the other waits for
@@ -23,20 +28,21 @@ constexpr int LN_MAX_COLS = 16384;  // the widest row held in registers
 // (131072 x 512: 128 us, 6300 GB/s, against 142 in two), two for 16 bits, bound by its instructions (131072 x 1024:
 // 133 us against 166).
 __host__ __device__ constexpr int ln_threads(int lanes, int e, bool backward) {
-  return lanes >= 512 ? lanes : !backward && (e == 4 || lanes <= 32) ? 512 : 256;
+  return lanes > LN_LANES || (!backward && lanes < LN_LANES && (e == 4 || lanes <= 32)) ? 512 : 256;
 }
-__host__ __device__ constexpr int ln_per_sm(int lanes, int e, bool backward) {
-  return ln_threads(lanes, e, backward) == 256 && !(backward && e == 4) ? 2 : 1;
+__host__ __device__ constexpr int ln_per_sm(int lanes, int e, bool backward, bool split) {
+  return ln_threads(lanes, e, backward) == 256 && (split || !(backward && e == 4)) ? 2 : 1;
 }
 
 // How a tensor's rows lie: SPAN: dense rows from a 16-byte boundary; PIECES: every row a whole number of 16-byte
 // pieces from a 16-byte boundary; VALUES: anything else.
 enum LnRows { SPAN = 0, PIECES = 1, VALUES = 2 };
 
-// The tiles of a call: rows of a tile, the tile's bytes in a stage (per tensor) and a stage's bytes.
+// The tiles of a call: rows of a tile, the tile's bytes in a stage (per tensor) and a stage's bytes. A row's columns
+// are split over `split` blocks, `width` to each (the last has what is left).
 struct LnTiles {
   long long rows;
-  int cols, lanes, ept, per_tile, stages, tile_bytes, stage_bytes;
+  int cols, split, width, lanes, ept, per_tile, stages, tile_bytes, stage_bytes;
 };
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src) {
@@ -62,12 +68,13 @@ template <class T, int THREADS> struct LnFeed {
   const T* next;  // the first row of the next tile
   int kind, cols;
   long long stride, step;  // in values: between rows, between the block's tiles
-  __device__ __forceinline__ LnFeed(const T* x, int kind, long long stride, const LnTiles& t, int cols)
-      : next(x + (long long)blockIdx.x * t.per_tile * stride),
+  __device__ __forceinline__ LnFeed(const T* x, int kind, long long stride, const LnTiles& t, int team, int teams,
+                                    int cols)
+      : next(x + (long long)team * t.per_tile * stride),
         kind(kind),
         cols(cols),
         stride(stride),
-        step((long long)gridDim.x * t.per_tile * stride) {}
+        step((long long)teams * t.per_tile * stride) {}
   // The byte at which the first row of the tile at p starts in its stage.
   __device__ __forceinline__ int phase(const T* p) const {
     return kind == SPAN ? (int)(reinterpret_cast<uintptr_t>(p) & 15) : 0;
@@ -84,10 +91,16 @@ template <class T, int THREADS> struct LnFeed {
         for (int i = pieces * P + threadIdx.x; i < bytes / (int)sizeof(T); i += THREADS)
           reinterpret_cast<T*>(dst)[i] = reinterpret_cast<const T*>(from)[i];
     } else if (kind == PIECES) {
-      const int per_row = cols / P, pieces = per_row * n;
-      for (int i = threadIdx.x; i < pieces; i += THREADS) {
-        const int r = i / per_row;
-        copy_async16(dst + i * 16, next + r * stride + (i - r * per_row) * P);
+      const int per_row = cols / P;
+      if (per_row >= THREADS) {
+        for (int r = 0; r < n; r++)
+          for (int i = threadIdx.x; i < per_row; i += THREADS)
+            copy_async16(dst + (r * per_row + i) * 16, next + r * stride + i * P);
+      } else {
+        for (int i = threadIdx.x; i < per_row * n; i += THREADS) {
+          const int r = i / per_row;
+          copy_async16(dst + i * 16, next + r * stride + (i - r * per_row) * P);
+        }
       }
     } else {
       for (int r = threadIdx.x >> 5; r < n; r += THREADS / 32) {
@@ -105,47 +118,89 @@ template <class T, int THREADS> struct LnFeed {
   }
 };
 
-// A block's tiles: the first row of the tile that is worked on, and of the one that is filled.
+// A block's (or cluster's) tiles: the first row of the tile that is worked on, and of the one that is filled.
 struct LnTurn {
   long long rows, row, fill_row, step;
   int per_tile;
-  __device__ __forceinline__ explicit LnTurn(const LnTiles& t)
+  __device__ __forceinline__ LnTurn(const LnTiles& t, int team, int teams)
       : rows(t.rows),
-        row((long long)blockIdx.x * t.per_tile),
+        row((long long)team * t.per_tile),
         fill_row(row),
-        step((long long)gridDim.x * t.per_tile),
+        step((long long)teams * t.per_tile),
         per_tile(t.per_tile) {}
   __device__ __forceinline__ int here(long long at) const {
     return rows - at < per_tile ? (int)(rows - at) : per_tile;
   }
 };
 
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_barrier() {
+  cluster_arrive();
+  cluster_wait();
+}
+
 // The LANES threads that share a row, and the sums of one or two floats over them: shuffles inside a warp, and for
-// wider rows one exchange through `slots` (two sets in turn, so one barrier is enough) under the group's own named
-// barrier. A thread holds the row's values i = 0 .. EPT - 1 at the columns (i / V * LANES + lane) * V + i % V, in pairs.
-template <int LANES> struct LnGroup {
+// wider rows one exchange through `slots` (two sets in turn, so one barrier is enough): under the group's own named
+// barrier, or, where the row is split over a cluster, with every warp's sum put into the slots of all its blocks, under
+// the cluster's barrier. A thread holds the row's values i = 0 .. EPT - 1 at the columns (i / V * LANES + lane) * V +
+// i % V, in pairs.
+template <int LANES, bool SPLIT> struct LnGroup {
   static constexpr int WARPS = LANES / 32;
   int lane, index;  // lane: the thread's place in its row's group; index: the group in the block
-  float2* slots;    // 2 x 32
+  int rank, split;  // of the cluster
+  float* slots;     // 2 x 64
   int turn;
-  template <int N> __device__ __forceinline__ void sum(float (&v)[N]) {
+  __device__ __forceinline__ void sum(float (&v)[1]) {
 #pragma unroll
-    for (int m = (LANES < 32 ? LANES : 32) / 2; m > 0; m >>= 1)
-#pragma unroll
-      for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
-    if constexpr (LANES > 32) {
-      float2* s = slots + (turn & 1) * 32 + index * WARPS;
+    for (int m = (LANES < 32 ? LANES : 32) / 2; m > 0; m >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+    if constexpr (SPLIT) {
+      float* s = slots + (turn & 1) * 64;
       turn++;
-      if ((threadIdx.x & 31) == 0) s[lane >> 5] = make_float2(v[0], v[N - 1]);
+      const int to = threadIdx.x & 31;  // lane k of each warp tells block k
+      if (to < split) {
+        unsigned at = (unsigned)__cvta_generic_to_shared(s + rank * WARPS + (lane >> 5));
+        asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(to));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v[0]) : "memory");
+      }
+      cluster_barrier();
+      const int all = split * WARPS;  // 16, 32 or 64
+      v[0] = s[to & (all - 1)];
+      if (all > 32) v[0] += s[32 + to];
+      for (int m = (all < 32 ? all : 32) / 2; m > 0; m >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+    } else if constexpr (LANES > 32) {
+      float* s = slots + (turn & 1) * 64 + index * WARPS;
+      turn++;
+      if ((threadIdx.x & 31) == 0) s[lane >> 5] = v[0];
       asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "n"(LANES) : "memory");
-      const float2 o = s[threadIdx.x & (WARPS - 1)];
-      v[0] = o.x;
-      v[N - 1] = N == 1 ? o.x : o.y;
+      v[0] = s[threadIdx.x & (WARPS - 1)];
 #pragma unroll
-      for (int m = WARPS / 2; m > 0; m >>= 1)
-#pragma unroll
-        for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
+      for (int m = WARPS / 2; m > 0; m >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
     }
+  }
+  // two sums: from the first step on half of a warp holds the one and half the other
+  __device__ __forceinline__ void sum(float (&v)[2]) {
+    static_assert(!SPLIT, "one sum at a time over a cluster");
+    constexpr int HALF = (LANES < 32 ? LANES : 32) / 2;
+    const bool upper = threadIdx.x & HALF;
+    float mine = upper ? v[1] : v[0];
+    mine += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[1], HALF);
+#pragma unroll
+    for (int m = HALF / 2; m > 0; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
+    if constexpr (LANES > 32) {
+      float* s = slots + (turn & 1) * 64 + index * 2 * WARPS + (upper ? WARPS : 0);
+      turn++;
+      if ((threadIdx.x & 15) == 0) s[lane >> 5] = mine;
+      asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "n"(LANES) : "memory");
+      mine = s[threadIdx.x & (WARPS - 1)];
+#pragma unroll
+      for (int m = WARPS / 2; m > 0; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, mine, HALF);
+    v[0] = upper ? other : mine;
+    v[1] = upper ? mine : other;
   }
 };
 
@@ -155,15 +210,16 @@ template <int LANES, int V> __device__ __forceinline__ int ln_column(int lane, i
 
 // A thread's values of a parameter, `absent` where there is none.
 template <int LANES, int EPT, int V>
-__device__ __forceinline__ void load_param(const void* p, int wtype, float absent, int cols, int lane, float2* out) {
+__device__ __forceinline__ void load_param(const void* p, int wtype, int col0, float absent, int cols, int lane,
+                                           float2* out) {
 #pragma unroll
   for (int i = 0; i < EPT; i++) {
     const int c = ln_column<LANES, V>(lane, i);
     float v = absent;
     if (p && c < cols)
-      v = wtype == F32 ? static_cast<const float*>(p)[c]
-          : wtype == BF16 ? to_f32(static_cast<const __nv_bfloat16*>(p)[c])
-                          : to_f32(static_cast<const __half*>(p)[c]);
+      v = wtype == F32 ? static_cast<const float*>(p)[col0 + c]
+          : wtype == BF16 ? to_f32(static_cast<const __nv_bfloat16*>(p)[col0 + c])
+                          : to_f32(static_cast<const __half*>(p)[col0 + c]);
     (i % 2 ? out[i / 2].y : out[i / 2].x) = v;
   }
 }
@@ -204,6 +260,23 @@ __device__ __forceinline__ void store_row(T* row, int cols, int lane, const floa
 }
 
 // Set the places beyond the last column to 0.
+// A thread's float32 values at its columns of `row` (any alignment of its start where V is 1 or 2).
+template <int LANES, int EPT, int V, bool FULL>
+__device__ __forceinline__ void store_sums(float* row, int cols, int lane, const float2* v) {
+#pragma unroll
+  for (int j = 0; j < EPT / V; j++) {
+    const int c = (j * LANES + lane) * V;
+    if (!FULL && c >= cols) continue;
+    if constexpr (V >= 4) {
+#pragma unroll
+      for (int k = 0; k < V / 4; k++) store_pairs<float, 4>(row + c + 4 * k, v + (j * V + 4 * k) / 2);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; k++) row[c + k] = (j * V + k) % 2 ? v[(j * V + k) / 2].y : v[(j * V + k) / 2].x;
+    }
+  }
+}
+
 template <int LANES, int EPT, int V>
 __device__ __forceinline__ void clear_beyond(int cols, int lane, float2* v) {
 #pragma unroll
@@ -211,22 +284,29 @@ __device__ __forceinline__ void clear_beyond(int cols, int lane, float2* v) {
     if (ln_column<LANES, V>(lane, i) >= cols) (i % 2 ? v[i / 2].y : v[i / 2].x) = 0.f;
 }
 
-// FULL: cols = LANES * EPT (no thread has a place beyond the last column)
-template <class T, int LANES, int EPT, int V, bool FULL>
-__global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm(LANES, sizeof(T), false))
+// FULL: every block has LANES * EPT columns (no thread has a place beyond the last); SPLIT: a row is split over the
+// blocks of a cluster
+template <class T, int LANES, int EPT, int V, bool FULL, bool SPLIT>
+__global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm(LANES, sizeof(T), false, SPLIT))
     k_ln_forward(LnTiles t, int kind, long long stride, const T* __restrict__ x, int wtype,
                  const void* __restrict__ weight, const void* __restrict__ bias, float eps, T* __restrict__ y,
                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float2 slots[64];
+  __shared__ float slots[128];
   constexpr int THREADS = ln_threads(LANES, sizeof(T), false), GROUPS = THREADS / LANES, N2 = EPT / 2;
-  const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
+  static_assert(!SPLIT || GROUPS == 1, "the blocks of a cluster share one row");
+  // this block's place in its cluster, its columns, and its team's place among the teams that take the tiles in turn
+  const int split = SPLIT ? t.split : 1, rank = SPLIT ? (int)(blockIdx.x % split) : 0, col0 = rank * t.width;
+  const int cols = FULL ? LANES * EPT : SPLIT ? min(t.width, t.cols - col0) : t.cols, pitch = SPLIT ? t.cols : cols;
+  const int team = SPLIT ? blockIdx.x / split : blockIdx.x, teams = SPLIT ? gridDim.x / split : gridDim.x;
+  const int lane = threadIdx.x % LANES;
   let_next_start();
-  LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
+  if (SPLIT) cluster_barrier();  // (the other blocks' slots are there)
+  LnGroup<LANES, SPLIT> g = {lane, (int)threadIdx.x / LANES, rank, split, slots, 0};
   const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;  // the group's place in its warp
-  const float inv = 1.f / cols;
-  LnFeed<T, THREADS> feed(x, kind, stride, t, cols);
-  LnTurn turn(t);
+  const float inv = 1.f / t.cols;
+  LnFeed<T, THREADS> feed(x + col0, kind, stride, t, team, teams, cols);
+  LnTurn turn(t, team, teams);
   auto fill = [&](int stage) {
     if (turn.fill_row < turn.rows) {
       const int n = turn.here(turn.fill_row);
@@ -236,13 +316,13 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
     copy_commit();
   };
   const T* at = feed.next;
-  T* out = y + turn.row * cols;
-  const long long out_step = turn.step * cols;
+  T* out = y + turn.row * pitch + col0;
+  const long long out_step = turn.step * pitch;
   wait_for_last();
   for (int s = 0; s + 1 < t.stages; s++) fill(s);
   float2 w[N2], b[N2];
-  load_param<LANES, EPT, V>(weight, wtype, 1.f, cols, lane, w);
-  load_param<LANES, EPT, V>(bias, wtype, 0.f, cols, lane, b);
+  load_param<LANES, EPT, V>(weight, wtype, col0, 1.f, cols, lane, w);
+  load_param<LANES, EPT, V>(bias, wtype, col0, 0.f, cols, lane, b);
   int stage = 0, free_stage = t.stages - 1;
   for (; turn.row < turn.rows; turn.row += turn.step, at += feed.step, out += out_step) {
     copy_wait(t.stages - 2);
@@ -274,30 +354,31 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
 #pragma unroll
       for (int i = 0; i < N2; i++) v[i] = fma2(mul2(v[i], both(rstd)), w[i], b[i]);
       if (r < n) {
-        store_row<T, LANES, EPT, V, FULL>(out + r * cols, cols, lane, v);
-        if (lane < 2) (lane ? rstd_out : mean_out)[turn.row + r] = lane ? rstd : mean;
+        store_row<T, LANES, EPT, V, FULL>(out + (long long)r * pitch, cols, lane, v);
+        if (rank == 0 && lane < 2) (lane ? rstd_out : mean_out)[turn.row + r] = lane ? rstd : mean;
       }
     }
   }
+  if (SPLIT) cluster_barrier();  // (nobody leaves while others put sums into its slots)
 }
 
 // part (gridDim.x, 2, cols), if wanted: the block's column sums of g xh and g
-// FULL: cols = LANES * EPT (no thread has a place beyond the last column)
 template <class T, int LANES, int EPT, int V, bool FULL>
-__global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(LANES, sizeof(T), true))
+__global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(LANES, sizeof(T), true, false))
     k_ln_backward(LnTiles t, int gkind, long long gstride, int kind, long long stride, const T* __restrict__ gy,
                   const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd, int wtype,
                   const void* __restrict__ weight, T* __restrict__ gx, float* __restrict__ part) {
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float2 slots[64];
+  __shared__ float slots[128];
   constexpr int THREADS = ln_threads(LANES, sizeof(T), true), GROUPS = THREADS / LANES, N2 = EPT / 2;
   const int cols = FULL ? LANES * EPT : t.cols, lane = threadIdx.x % LANES;
   let_next_start();
-  LnGroup<LANES> g = {lane, (int)threadIdx.x / LANES, slots, 0};
+  LnGroup<LANES, false> g = {lane, (int)threadIdx.x / LANES, 0, 1, slots, 0};
   const int shift = LANES < 32 ? (int)(threadIdx.x & 31) / LANES : 0;
-  const float inv = 1.f / cols;
-  LnFeed<T, THREADS> xfeed(x, kind, stride, t, cols), gfeed(gy, gkind, gstride, t, cols);
-  LnTurn turn(t);
+  const float inv = 1.f / t.cols;
+  LnFeed<T, THREADS> xfeed(x, kind, stride, t, blockIdx.x, gridDim.x, cols);
+  LnFeed<T, THREADS> gfeed(gy, gkind, gstride, t, blockIdx.x, gridDim.x, cols);
+  LnTurn turn(t, blockIdx.x, gridDim.x);
   auto fill = [&](int stage) {
     if (turn.fill_row < turn.rows) {
       unsigned char* to = ring + stage * t.stage_bytes;
@@ -320,7 +401,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
   wait_for_last();
   for (int s = 0; s + 1 < t.stages; s++) fill(s);
   float2 w[N2], gw[N2], gb[N2];
-  load_param<LANES, EPT, V>(weight, wtype, 1.f, cols, lane, w);
+  load_param<LANES, EPT, V>(weight, wtype, 0, 1.f, cols, lane, w);
 #pragma unroll
   for (int i = 0; i < N2; i++) gw[i] = gb[i] = both(0.f);
   int stage = 0, free_stage = t.stages - 1;
@@ -361,10 +442,10 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
       float c[2] = {c1.x + c1.y, c2.x + c2.y};
       g.sum(c);
       if (!gx || r >= n) continue;
-      c1 = both(-c[0] * inv);
-      c2 = both(-c[1] * inv);
+      c1 = both(-c[0] * inv * rs);
+      c2 = both(-c[1] * inv * rs);
 #pragma unroll
-      for (int i = 0; i < N2; i++) h[i] = mul2(add2(fma2(xh[i], c2, h[i]), c1), both(rs));
+      for (int i = 0; i < N2; i++) h[i] = fma2(xh[i], c2, fma2(h[i], both(rs), c1));
       store_row<T, LANES, EPT, V, FULL>(out + r * cols, cols, lane, h);
     }
   }
@@ -376,14 +457,8 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
     copy_wait(0);
     __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < EPT; i++) {
-    const int c = ln_column<LANES, V>(lane, i);
-    if (FULL || c < cols) {
-      mine[c] = i % 2 ? gw[i / 2].y : gw[i / 2].x;
-      mine[cols + c] = i % 2 ? gb[i / 2].y : gb[i / 2].x;
-    }
-  }
+  store_sums<LANES, EPT, V, FULL>(mine, cols, lane, gw);
+  store_sums<LANES, EPT, V, FULL>(mine + cols, cols, lane, gb);
   if (GROUPS == 1) return;
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * cols; c += THREADS) {
@@ -392,6 +467,132 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
     for (int k = 0; k < GROUPS; k++) v += reinterpret_cast<const float*>(ring)[k * 2 * cols + c];
     sums[c] = v;
   }
+}
+
+// The backward of rows that one block does not take: a row to each team of t.split blocks (a cluster) of LANES threads,
+// t.width columns to a block. The two sums of a row meet in the slots of all its blocks
+// under the cluster's barrier, which is split: between arriving with row k's sums and waiting for the others' a thread
+// finishes row k - 1, from shared memory again: nobody stands still for the exchange, for half as many instructions
+// again (8192 x 8192 bfloat16, which needs no cluster, takes 103 us here and 94 in k_ln_backward). part (teams, 2,
+// cols), if wanted.
+template <class T, int LANES, int V, bool FULL>
+__global__ void __launch_bounds__(LANES, 512 / LANES)
+    k_ln_backward_split(LnTiles t, int gkind, long long gstride, int kind, long long stride, const T* __restrict__ gy,
+                        const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
+                        int wtype, const void* __restrict__ weight, T* __restrict__ gx, float* __restrict__ part) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float2 slots[2][128];
+  constexpr int EPT = ln_split_ept(sizeof(T)), N2 = EPT / 2, WARPS = LANES / 32;
+  const int split = t.split, rank = blockIdx.x % split, team = blockIdx.x / split, teams = gridDim.x / split;
+  const int col0 = rank * t.width, cols = FULL ? LANES * EPT : min(t.width, t.cols - col0);
+  const int lane = threadIdx.x, to = lane & 31, all = split * WARPS;
+  let_next_start();
+  LnFeed<T, LANES> xfeed(x + col0, kind, stride, t, team, teams, cols);
+  LnFeed<T, LANES> gfeed(gy + col0, gkind, gstride, t, team, teams, cols);
+  const float inv = 1.f / t.cols;
+  long long fill_row = team;
+  auto fill = [&](int stage) {
+    if (fill_row < t.rows) {
+      unsigned char* dst = ring + stage * t.stage_bytes;
+      xfeed.fill(dst, 1, fill_row + 1 == t.rows);
+      gfeed.fill(dst + t.tile_bytes, 1, fill_row + 1 == t.rows);
+      float* stats = reinterpret_cast<float*>(dst + 2 * t.tile_bytes);
+      if (lane < 2) copy_async4(stats + lane, (lane ? rstd : mean) + fill_row);
+      fill_row += teams;
+    }
+    copy_commit();
+  };
+  const T *xat = xfeed.next, *gat = gfeed.next;
+  cluster_arrive();
+  wait_for_last();
+  for (int s = 0; s + 2 < t.stages; s++) fill(s);
+  float2 w[N2], gw[N2], gb[N2];
+  load_param<LANES, EPT, V>(weight, wtype, col0, 1.f, cols, lane, w);
+#pragma unroll
+  for (int i = 0; i < N2; i++) gw[i] = gb[i] = both(0.f);
+  copy_wait(t.stages - 3);  // row 0 is here
+  __syncthreads();
+  cluster_wait();  // (and the other blocks' slots are there)
+  // a row of stage `stage`: its normalised values and its cotangent times the weight
+  auto load = [&](int stage, const T* xp, const T* gp, float2* xh, float2* h) {
+    const unsigned char* base = ring + stage * t.stage_bytes;
+    load_row<T, LANES, EPT, V, FULL>(reinterpret_cast<const T*>(base + xfeed.phase(xp)), cols, lane, xh);
+    load_row<T, LANES, EPT, V, FULL>(reinterpret_cast<const T*>(base + t.tile_bytes + gfeed.phase(gp)), cols, lane, h);
+    const float* stats = reinterpret_cast<const float*>(base + 2 * t.tile_bytes);
+    const float m = stats[0], rs = stats[1];
+#pragma unroll
+    for (int i = 0; i < N2; i++) xh[i] = mul2(add2(xh[i], both(-m)), both(rs));
+    if (!FULL) clear_beyond<LANES, EPT, V>(cols, lane, xh);
+    return rs;
+  };
+  int stage = 0, last = 0, next = t.stages - 2;  // of the row that is summed, of the one that is finished, to be filled
+  float c1 = 0.f, c2 = 0.f;
+  T* out = gx + (long long)team * t.cols + col0;  // of the row that is finished
+  auto finish = [&](int at, const T* xp, const T* gp) {
+    if (!gx) return;
+    float2 xh[N2], h[N2];
+    const float rs = load(at, xp, gp, xh, h);
+    const float2 a = both(-c1 * inv * rs), b = both(-c2 * inv * rs);
+#pragma unroll
+    for (int i = 0; i < N2; i++) h[i] = fma2(xh[i], b, fma2(mul2(h[i], w[i]), both(rs), a));
+    store_row<T, LANES, EPT, V, FULL>(out, cols, lane, h);
+    out += (long long)teams * t.cols;
+  };
+  bool first = true;
+  int turn = 0;
+  for (long long row = team; row < t.rows; row += teams, turn ^= 1) {
+    float s[2];
+    {
+      float2 xh[N2], h[N2], a = both(0.f), b = both(0.f);
+      load(stage, xat, gat, xh, h);
+#pragma unroll
+      for (int i = 0; i < N2; i++) {
+        gw[i] = fma2(h[i], xh[i], gw[i]);
+        gb[i] = add2(gb[i], h[i]);
+        h[i] = mul2(h[i], w[i]);
+        a = add2(a, h[i]);
+        b = fma2(h[i], xh[i], b);
+      }
+      s[0] = a.x + a.y;
+      s[1] = b.x + b.y;
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], m);
+      s[1] += __shfl_xor_sync(0xffffffffu, s[1], m);
+    }
+    if (to < split) {  // lane k of each warp tells block k
+      unsigned at = (unsigned)__cvta_generic_to_shared(&slots[turn][rank * WARPS + (lane >> 5)]);
+      asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(to));
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(s[0]), "f"(s[1]) : "memory");
+    }
+    copy_wait(t.stages - 4);  // the next row is here once everybody has arrived
+    __syncwarp();
+    cluster_arrive();
+    if (!first) finish(last, xat - xfeed.step, gat - gfeed.step);
+    first = false;
+    cluster_wait();
+    // the sums of this row (read before the next arrival: the slots are the next but one row's), and the stage of the
+    // row before the last, which everybody has finished
+    float2 o = slots[turn][to & (all - 1)];
+    for (int k = 32 + to; k < all; k += 32) o.x += slots[turn][k].x, o.y += slots[turn][k].y;
+    for (int m = (all < 32 ? all : 32) / 2; m > 0; m >>= 1) {
+      o.x += __shfl_xor_sync(0xffffffffu, o.x, m);
+      o.y += __shfl_xor_sync(0xffffffffu, o.y, m);
+    }
+    c1 = o.x, c2 = o.y;
+    fill(next);
+    next = next + 1 == t.stages ? 0 : next + 1;
+    last = stage;
+    stage = stage + 1 == t.stages ? 0 : stage + 1;
+    xat += xfeed.step, gat += gfeed.step;
+  }
+  if (!first) finish(last, xat - xfeed.step, gat - gfeed.step);
+  copy_wait(0);
+  if (!part) return;
+  float* sums = part + (long long)team * 2 * t.cols + col0;
+  store_sums<LANES, EPT, V, FULL>(sums, cols, lane, gw);
+  store_sums<LANES, EPT, V, FULL>(sums + t.cols, cols, lane, gb);
 }
 
 // gw, gb = the sums of the blocks' column sums: 32 columns a block, a warp for each WARPS-th of the parts

@@ -5,11 +5,11 @@ namespace nbtrain {
 
 long long ln_max_parts(long long rows, int cols) {
   const int wide = ln_wide_parts(rows);
-  if (cols > LN_MAX_COLS) return wide;
-  int lanes, ept;
-  ln_spread(cols, true, &lanes, &ept);
-  const long long blocks = (rows * lanes + 255) / 256;  // (blocks of 256 threads or more, two per SM at most)
-  return std::max<long long>(std::min<long long>(blocks, 2 * SMS), wide);
+  if (cols > LN_WIDEST) return wide;
+  LnTiles t;  // (the teams of either value size: rows / groups, two blocks per SM at most)
+  ln_spread(cols, 4, true, &t);
+  const long long teams = (rows * t.lanes + 255) / 256;
+  return std::max<long long>(std::min<long long>(teams, 2 * SMS), wide);
 }
 
 template int ln_forward<float>(const LnForward& a);

@@ -10,43 +10,52 @@
 
 namespace nbtrain {
 
-// How a layer norm of rows that a ring holds is spread: the tiles, and the blocks that take the tiles in turn.
-constexpr int LN_SMEM = 226 * 1024, LN_SMEM_SM = 220 * 1024;
-// bytes of a tile: 48 KB, or 32 where the backward's two tensors or two blocks an SM share the stages
-constexpr int ln_tile(int lanes, bool backward) { return backward && lanes < 512 ? 32768 : backward ? 65536 : 49152; }
+// How a layer norm of rows that a ring holds is spread: the tiles, and the blocks (clusters) that take them in turn.
+constexpr int LN_SMEM = 224 * 1024, LN_SMEM_SM = 220 * 1024;
+// bytes of a tile, of all tensors (131072 x 512 float32 backward: 128 us with 32 KB, 146 with 64; 8192 x 8192 bfloat16,
+// whose one block an SM waits at each tile: 88 us with 64, 97 with 32)
+constexpr int ln_tile(int lanes, bool backward) { return !backward ? 49152 : lanes > LN_LANES ? 65536 : 32768; }
 struct LnPlan {
   LnTiles t;
-  int blocks, smem;
+  int blocks, smem, per_sm;
   bool fits;
 };
-// The lanes of a row and the values per lane.
-inline void ln_spread(int cols, bool backward, int* lanes, int* ept) {
-  // 8 for the narrowest rows, where 16 would leave half of the places empty (36 columns of float32: see k_ln_forward);
-  // 32 for the widest of the forward, whose sums then meet in 8 warps instead of 16 (8192 x 8192 bfloat16: 49 us
-  // against 59; the backward's two column sums leave no registers for it)
-  *ept = cols <= 64 ? 8 : !backward && cols > 4096 ? 32 : 16;
-  *lanes = 8;
-  while (*lanes * *ept < cols) *lanes *= 2;
+// The blocks and lanes of a row and the values per lane. 8 values for the narrowest rows, where 16 would leave half of
+// the places empty; 32 for the widest of the forward, whose sums then meet in 8 warps instead of 16 (8192 x 8192
+// bfloat16: 49 us against 59; the backward's column sums leave no registers for it, so it takes 512 lanes there).
+// Beyond that a row is split over a cluster, evenly and in multiples of 16 columns, so that every part keeps the row's
+// alignment.
+inline bool ln_split_rows(int cols) { return cols > 16 * LN_SPLIT_LANES; }  // (in the backward)
+inline void ln_spread(int cols, int e, bool backward, LnTiles* t) {
+  const bool wide = cols > 16 * LN_LANES;
+  const int most = backward && wide ? LN_SPLIT_LANES : LN_LANES;
+  t->ept = cols <= 64 ? 8 : wide && !backward ? 32 : backward && ln_split_rows(cols) ? ln_split_ept(e) : 16;
+  t->split = 1;
+  while (t->split * most * t->ept < cols) t->split *= 2;
+  t->width = t->split == 1 ? cols : ((cols + t->split - 1) / t->split + 15) / 16 * 16;
+  t->lanes = wide ? most : 8;
+  while (t->lanes * t->ept < t->width) t->lanes *= 2;
 }
 inline LnPlan ln_plan(long long rows, int cols, int e, bool backward) {
   LnPlan p = {};
-  p.fits = cols <= LN_MAX_COLS;
+  p.fits = cols <= LN_WIDEST;
   if (!p.fits) return p;
-  ln_spread(cols, backward, &p.t.lanes, &p.t.ept);
-  const int lanes = p.t.lanes, groups = ln_threads(lanes, e, backward) / lanes, row = cols * e;
-  const int per_sm = ln_per_sm(lanes, e, backward), tensors = backward ? 2 : 1;
-  const long long slots = (long long)SMS * per_sm, rounds = (rows + groups - 1) / groups;
-  // a tile of about ln_tile bytes (of all tensors), but not so long that a block has no tile
-  const int per_group = (int)std::max<long long>(
+  ln_spread(cols, e, backward, &p.t);
+  const int lanes = p.t.lanes, row = p.t.width * e, tensors = backward ? 2 : 1;
+  const int groups = ln_threads(lanes, e, backward) / lanes;
+  const bool split = backward && ln_split_rows(cols);  // (tiles of one row, and more of them)
+  p.per_sm = ln_per_sm(lanes, e, backward, p.t.split > 1);
+  const long long slots = (long long)SMS * p.per_sm / p.t.split, rounds = (rows + groups - 1) / groups;
+  // a tile of about ln_tile bytes, but not so long that a block has no tile
+  const int per_group = split ? 1 : (int)std::max<long long>(
       1, std::min<long long>(ln_tile(lanes, backward) / (groups * row * tensors), (rounds + slots - 1) / slots));
   p.t.rows = rows, p.t.cols = cols, p.t.per_tile = groups * per_group;
   p.t.tile_bytes = (p.t.per_tile * row + 15) / 16 * 16 + 16;  // (16: a first row that starts inside a piece)
   p.t.stage_bytes = tensors * p.t.tile_bytes + (backward ? (8 * p.t.per_tile + 15) / 16 * 16 : 0);
-  p.t.stages = std::min(4, LN_SMEM_SM / per_sm / p.t.stage_bytes);
-  if (p.t.stages < 2) p.t.stages = std::min(4, LN_SMEM / p.t.stage_bytes);
-  p.fits = p.t.stages >= 2;
+  p.t.stages = std::min(split ? 6 : 4, LN_SMEM_SM / p.per_sm / p.t.stage_bytes);
+  p.fits = p.t.stages >= (split ? 4 : 2);
   p.smem = p.t.stages * p.t.stage_bytes;
-  p.blocks = (int)std::min<long long>((rounds + per_group - 1) / per_group, slots);
+  p.blocks = (int)std::min<long long>((rounds + per_group - 1) / per_group, slots) * p.t.split;
   return p;
 }
 
@@ -54,10 +63,11 @@ inline LnPlan ln_plan(long long rows, int cols, int e, bool backward) {
 constexpr int LN_WIDE_PARTS = 64;
 inline int ln_wide_parts(long long rows) { return (int)std::min<long long>(LN_WIDE_PARTS, (rows + 15) / 16); }
 
-inline int ln_kind(const void* p, long long rows, int cols, long long stride, int e) {
-  if (rows == 1) stride = cols;
+inline int ln_kind(const void* p, const LnTiles& t, long long stride, int e) {
+  const int cols = t.cols;
+  if (t.rows == 1) stride = cols;
   const bool start = reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  if (start && stride == cols) return SPAN;
+  if (start && stride == cols && t.split == 1) return SPAN;
   return start && (long long)cols * e % 16 == 0 && stride * e % 16 == 0 ? PIECES : VALUES;
 }
 
@@ -67,46 +77,85 @@ inline int ln_vector(int e, int cols, const void* result) {
   return bits % 16 == 0 ? 16 / e : bits % 4 == 0 ? 4 / e : 1;
 }
 
-// calls f with the lanes of a row, the values per lane, the vector length and whether the lanes' places are all taken,
-// as types
+// calls f with the lanes of a row, the values per lane, the vector length, whether the lanes' places are all taken and
+// whether the row is split, as types
 template <int N> using Int = std::integral_constant<int, N>;
 template <class T, class F> int ln_vectors(const LnTiles& t, int vector, F f) {
   if (vector == (int)(16 / sizeof(T)))
-    return t.cols == t.lanes * t.ept ? f(Int<16 / sizeof(T)>(), std::true_type())
-                                     : f(Int<16 / sizeof(T)>(), std::false_type());
+    return t.cols == t.split * t.lanes * t.ept ? f(Int<16 / sizeof(T)>(), std::true_type())
+                                               : f(Int<16 / sizeof(T)>(), std::false_type());
   if (sizeof(T) == 2 && vector == 2) return f(Int<4 / sizeof(T)>(), std::false_type());
   return f(Int<1>(), std::false_type());
 }
 template <class T, bool BACKWARD, class F> int ln_variant(const LnTiles& t, int vector, F f) {
-  auto with = [&](auto lanes, auto ept) {
-    return ln_vectors<T>(t, vector, [&](auto v, auto full) { return f(lanes, ept, v, full); });
+  auto with = [&](auto lanes, auto ept, auto split) {
+    return ln_vectors<T>(t, vector, [&](auto v, auto full) { return f(lanes, ept, v, full, split); });
   };
+  const std::false_type one;
+  if constexpr (!BACKWARD)
+    if (t.split > 1) return with(Int<LN_LANES>(), Int<32>(), std::true_type());
+  if (t.ept == 8) return with(Int<8>(), Int<8>(), one);
+  if constexpr (!BACKWARD)
+    if (t.ept == 32) return with(Int<LN_LANES>(), Int<32>(), one);
   switch (t.lanes) {
-    case 8: return t.ept == 8 ? with(Int<8>(), Int<8>()) : with(Int<8>(), Int<16>());
-    case 16: return with(Int<16>(), Int<16>());
-    case 32: return with(Int<32>(), Int<16>());
-    case 64: return with(Int<64>(), Int<16>());
-    case 128: return with(Int<128>(), Int<16>());
-    case 256:
-      if constexpr (!BACKWARD)
-        if (t.ept == 32) return with(Int<256>(), Int<32>());
-      return with(Int<256>(), Int<16>());
-    case 512: return with(Int<512>(), Int<BACKWARD ? 16 : 32>());
+    case 8: return with(Int<8>(), Int<16>(), one);
+    case 16: return with(Int<16>(), Int<16>(), one);
+    case 32: return with(Int<32>(), Int<16>(), one);
+    case 64: return with(Int<64>(), Int<16>(), one);
+    case 128: return with(Int<128>(), Int<16>(), one);
+    case LN_LANES: return with(Int<LN_LANES>(), Int<16>(), one);
     default:
-      if constexpr (BACKWARD) return with(Int<1024>(), Int<16>());
+      if constexpr (BACKWARD) return with(Int<LN_SPLIT_LANES>(), Int<16>(), one);
       else return (int)cudaErrorInvalidValue;
   }
 }
 
+// The blocks of a call whose rows are split over clusters: no more than the GPU holds at a time (asked once per kernel,
+// cluster size and device).
+template <auto KERNEL> int cluster_blocks(const LnPlan& p, int threads) {
+  static std::atomic<int> known[64 * (LN_CLUSTER + 1)];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return p.blocks;
+  std::atomic<int>& held = known[dev * (LN_CLUSTER + 1) + p.t.split];
+  n = held.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.t.split, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(p.t.split * SMS);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = LN_SMEM_SM / p.per_sm;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &config) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      return p.blocks;  // (they run one after the other)
+    }
+    held.store(n, std::memory_order_relaxed);
+  }
+  return std::min(p.blocks, n * p.t.split);
+}
+
 // Lets a kernel use all of an SM's shared memory, once per device.
-template <class K> int allow_smem(K kernel, std::atomic<bool>* done) {
+template <auto KERNEL> int allow_smem() {
+  static std::atomic<bool> done[64];
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_relaxed)) return 0;
-  const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM);
+  const cudaError_t rc = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM);
   if (rc == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_relaxed);
   return (int)rc;
+}
+
+// Prepares KERNEL and launches it as the plan has it (`blocks` is set to how many there are).
+template <auto KERNEL, class... A>
+int ln_launch(cudaStream_t stream, const LnPlan& p, int threads, int* blocks, A... args) {
+  const int e = allow_smem<KERNEL>();
+  if (e) return e;
+  *blocks = p.t.split > 1 ? cluster_blocks<KERNEL>(p, threads) : p.blocks;
+  return launch_after({stream, *blocks, threads, p.smem, p.t.split}, KERNEL, p.t, args...);
 }
 
 // calls f with the value type of the parameters
@@ -128,14 +177,13 @@ template <class T> int ln_forward(const LnForward& a) {
     });
     return (int)cudaGetLastError();
   }
-  const int kind = ln_kind(a.x, a.rows, a.cols, a.stride, sizeof(T));
-  return ln_variant<T, false>(p.t, ln_vector(sizeof(T), a.cols, y), [&](auto lanes, auto ept, auto v, auto full) {
-    auto kernel = k_ln_forward<T, lanes.value, ept.value, v.value, full.value>;
-    static std::atomic<bool> done[64];
-    const int e = allow_smem(kernel, done);
-    if (e) return e;
-    return launch_after(a.stream, p.blocks, ln_threads(lanes.value, sizeof(T), false), p.smem, kernel, p.t, kind,
-                        a.stride, x, a.wtype, a.weight, a.bias, a.eps, y, a.mean, a.rstd);
+  const int kind = ln_kind(a.x, p.t, a.stride, sizeof(T));
+  int blocks;
+  return ln_variant<T, false>(p.t, ln_vector(sizeof(T), a.cols, y), [&](auto lanes, auto ept, auto v, auto full,
+                                                                       auto split) {
+    return ln_launch<k_ln_forward<T, lanes.value, ept.value, v.value, full.value, split.value>>(
+        a.stream, p, ln_threads(lanes.value, sizeof(T), false), &blocks, kind, a.stride, x, a.wtype, a.weight, a.bias,
+        a.eps, y, a.mean, a.rstd);
   });
 }
 
@@ -158,25 +206,30 @@ template <class T> int ln_backward(const LnBackward& a) {
           a.rows, a.cols, a.g_stride, a.stride, g, x, a.mean, a.rstd, (a.rows + parts - 1) / parts, a.part);
     e = (int)cudaGetLastError();
   } else if (a.rows) {
-    parts = p.blocks;
-    const int gkind = ln_kind(a.g, a.rows, a.cols, a.g_stride, sizeof(T));
-    const int kind = ln_kind(a.x, a.rows, a.cols, a.stride, sizeof(T));
-    e = ln_variant<T, true>(p.t, ln_vector(sizeof(T), a.cols, gx), [&](auto lanes, auto ept, auto v, auto full) {
-      auto kernel = k_ln_backward<T, lanes.value, ept.value, v.value, full.value>;
-      static std::atomic<bool> done[64];
-      const int rc = allow_smem(kernel, done);
-      if (rc) return rc;
-      return launch_after(a.stream, p.blocks, ln_threads(lanes.value, sizeof(T), true), p.smem, kernel, p.t, gkind,
-                          a.g_stride, kind, a.stride, g, x, a.mean, a.rstd, a.wtype, a.weight, gx,
-                          sums ? a.part : nullptr);
-    });
+    const int gkind = ln_kind(a.g, p.t, a.g_stride, sizeof(T)), kind = ln_kind(a.x, p.t, a.stride, sizeof(T));
+    const int vector = ln_vector(sizeof(T), a.cols, gx);
+    float* part = sums ? a.part : nullptr;
+    int blocks = 0;
+    if (ln_split_rows(a.cols))
+      e = ln_vectors<T>(p.t, vector, [&](auto v, auto full) {
+        return ln_launch<k_ln_backward_split<T, LN_SPLIT_LANES, v.value, full.value>>(
+            a.stream, p, LN_SPLIT_LANES, &blocks, gkind, a.g_stride, kind, a.stride, g, x, a.mean, a.rstd, a.wtype,
+            a.weight, gx, part);
+      });
+    else
+      e = ln_variant<T, true>(p.t, vector, [&](auto lanes, auto ept, auto v, auto full, auto) {
+        return ln_launch<k_ln_backward<T, lanes.value, ept.value, v.value, full.value>>(
+            a.stream, p, ln_threads(lanes.value, sizeof(T), true), &blocks, gkind, a.g_stride, kind, a.stride, g, x,
+            a.mean, a.rstd, a.wtype, a.weight, gx, part);
+      });
+    parts = blocks / p.t.split;
   }
   if (e || !sums) return e;
   ln_param_type<T>(a.wtype, [&](auto w) {
     using W = decltype(w);
     // (many warps to a column where there are few columns, few where a block would wait for its place)
     auto sum = [&](auto warps) {
-      return launch_after(a.stream, (2 * a.cols + 31) / 32, 32 * warps.value, 0, k_ln_backward_sum<W, warps.value>,
+      return launch_after({a.stream, (2 * a.cols + 31) / 32, 32 * warps.value}, k_ln_backward_sum<W, warps.value>,
                           parts, a.cols, a.part, static_cast<W*>(a.gw), static_cast<W*>(a.gb));
     };
     e = a.cols <= 2048 ? sum(Int<32>()) : sum(Int<8>());

@@ -116,7 +116,7 @@ template <int N> int grad_sumsq(cudaStream_t stream, const GradList& g, double2*
     const int blocks = fill_table(t, i0, g.count, g.in, nullptr, g.sizes, g.types, nullptr);
     if (blocks < 0) return cudaErrorInvalidValue;
     if (!blocks) continue;
-    const int e = launch_after(stream, blocks, GN_THREADS, 0, k_grad_sumsq<N>, t, g.zero, *parts, part);
+    const int e = launch_after({stream, blocks, GN_THREADS}, k_grad_sumsq<N>, t, g.zero, *parts, part);
     if (e) return e;
     *parts += blocks;
   }
@@ -136,13 +136,13 @@ int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2*
     const int blocks = fill_table(t, i0, g.count, g.in, g.out, g.sizes, g.types, g.out_types);
     if (blocks < 0) return cudaErrorInvalidValue;
     if (!blocks) continue;
-    const int e = launch_after(stream, blocks, GN_THREADS, 0, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero,
+    const int e = launch_after({stream, blocks, GN_THREADS}, k_grad_scale<N>, t, parts, part, max_norm, eps, g.zero,
                                first ? norm : nullptr, first ? bad : nullptr);
     if (e) return e;
     first = false;
   }
   if (!first || (!norm && !bad)) return 0;
-  return launch_after(stream, 1, GN_THREADS, 0, k_grad_finish, parts, part, nullptr, norm, bad);
+  return launch_after({stream, 1, GN_THREADS}, k_grad_finish, parts, part, nullptr, norm, bad);
 }
 int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2* part, double max_norm, double eps,
                float* norm, long long* bad) {
@@ -203,7 +203,7 @@ int nb_g1_grad_sumsq(cudaStream_t stream, int count, const void* const* grads, c
   int parts = 0;
   const int e = grad_sumsq(stream, {count, grads, nullptr, sizes, types, nullptr, zero_nonfinite}, part, &parts);
   if (e) return e;
-  return launch_after(stream, 1, GN_THREADS, 0, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr,
+  return launch_after({stream, 1, GN_THREADS}, k_grad_finish, parts, part, reinterpret_cast<double2*>(stats), nullptr,
                       nullptr);
 }
 
