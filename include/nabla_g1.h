@@ -207,7 +207,10 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
  *     each where not NULL. An output may be its own gradient (same address and type); outputs that overlap anything
  *     else are refused. outs NULL: norm and bad alone.
  *   clip: sumsq, then scale.
- * work: nb_g1_grad_work_bytes(count) bytes, 16-byte aligned. */
+ * work: nb_g1_grad_work_bytes(count) bytes, 16-byte aligned; clip takes none (NULL) for a list of at most
+ * NB_G1_GRAD_SMALL_TENSORS tensors and NB_G1_GRAD_SMALL_VALUES values in all. */
+#define NB_G1_GRAD_SMALL_TENSORS 96
+#define NB_G1_GRAD_SMALL_VALUES 524288
 long long nb_g1_grad_work_bytes(int count);
 int nb_g1_grad_sumsq(cudaStream_t stream, int count, const void* const* grads, const long long* sizes,
                      const int* types, int zero_nonfinite, void* work, double* stats);

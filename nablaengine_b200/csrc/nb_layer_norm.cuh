@@ -133,15 +133,6 @@ struct LnTurn {
   }
 };
 
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_barrier() {
-  cluster_arrive();
-  cluster_wait();
-}
-
 // The LANES threads that share a row, and the sums of one or two floats over them: shuffles inside a warp, and for
 // wider rows one exchange through `slots` (two sets in turn, so one barrier is enough): under the group's own named
 // barrier, or, where the row is split over a cluster, with every warp's sum put into the slots of all its blocks, under

@@ -279,9 +279,12 @@ std::vector<Tensor> grad_clip(PyObject* const* a) {
   const Tensor norm = empty_on(g.device, {}, at::kFloat), bad = empty_on(g.device, {}, at::kLong);
   long long* badp = reinterpret_cast<long long*>(bad.data_ptr<int64_t>());
   if (a[5] == Py_None) {
-    const Tensor work = work_for(g);
+    long long values = 0;
+    for (long long n : g.sizes) values += n;
+    Tensor work;
+    if (count > NB_G1_GRAD_SMALL_TENSORS || values > NB_G1_GRAD_SMALL_VALUES) work = work_for(g);
     check(nb_g1_grad_clip(stream, count, g.at.data(), outs, g.sizes.data(), g.types.data(), o.types.data(), zero,
-                          max_norm, eps, work.data_ptr(), norm.data_ptr<float>(), badp),
+                          max_norm, eps, at_or_null(work), norm.data_ptr<float>(), badp),
           "nb_g1_grad_clip", OVERLAP);
   } else {
     const Tensor& stats = THPVariable_Unpack(a[5]);

@@ -2,6 +2,7 @@
 // layer norm (nb_layer_norm.cuh) and the global gradient norm with clipping (nb_grad_norm.cuh).
 #include "../../include/nabla_g1.h"
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -70,13 +71,13 @@ int grad_launches(int count) { return (count + GN_MANY - 1) / GN_MANY; }
 // The table of the tensors from i0 on, as many as it takes; returns its launch's blocks.
 template <int N>
 int fill_table(GradTable<N>& t, int i0, int count, const void* const* in, void* const* out, const long long* sizes,
-               const int* types, const int* out_types) {
+               const int* types, const int* out_types, int shortest = 2048, int takers = GN_BLOCKS) {
   const int i1 = std::min(count, i0 + N);
   long long total = 0, chunks = 0;
   for (int i = i0; i < i1; i++) total += sizes[i];
-  // chunks of 2048 to 16384 values: about one for each block where the tensors are small
-  t.chunk = 2048;
-  while (t.chunk < 16384 && total > (long long)t.chunk * GN_BLOCKS) t.chunk *= 2;
+  // chunks of `shortest` to 16384 values: about one for each block (or warp) that takes them where there are few
+  t.chunk = shortest;
+  while (t.chunk < 16384 && total > (long long)t.chunk * takers) t.chunk *= 2;
   t.count = 0;
   for (int i = i0; i < i1; i++) {
     if (sizes[i] == 0) continue;
@@ -149,6 +150,48 @@ int grad_scale(cudaStream_t stream, const GradList& g, int parts, const double2*
   return g.count <= GN_FEW ? grad_scale<GN_FEW>(stream, g, parts, part, max_norm, eps, norm, bad)
                            : grad_scale<GN_MANY>(stream, g, parts, part, max_norm, eps, norm, bad);
 }
+
+// A list that one cluster takes in one launch (measured: see k_grad_small).
+bool grad_small(int count, const long long* sizes) {
+  if (count > NB_G1_GRAD_SMALL_TENSORS) return false;
+  long long total = 0;
+  for (int i = 0; i < count; i++) total += sizes[i];
+  return total <= NB_G1_GRAD_SMALL_VALUES;
+}
+template <int BLOCKS>
+int grad_clip_small(cudaStream_t stream, const GradList& g, double max_norm, double eps, float* norm, long long* bad) {
+  GradTable<GN_FEW> t;
+  if (fill_table(t, 0, g.count, g.in, g.out, g.sizes, g.types, g.out_types, 512, BLOCKS * GN_SMALL_THREADS / 32) < 0)
+    return cudaErrorInvalidValue;
+  return launch_after({stream, BLOCKS, GN_SMALL_THREADS, 0, BLOCKS}, k_grad_small<BLOCKS>, t, g.out ? 1 : 0, max_norm,
+                      eps, g.zero, norm, bad);
+}
+// Whether the current device holds a cluster of 16 blocks of k_grad_small (8 is what every device does), asked once.
+bool cluster_of_16() {
+  static std::atomic<int> known[64];  // 0: not asked, 1: no, 2: yes
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  int k = known[dev].load(std::memory_order_relaxed);
+  if (k == 0) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 16, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(16);
+    config.blockDim = dim3(GN_SMALL_THREADS);
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    int n = 0;
+    const bool yes =
+        cudaFuncSetAttribute(k_grad_small<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&n, k_grad_small<16>, &config) == cudaSuccess && n > 0;
+    if (!yes) (void)cudaGetLastError();
+    k = yes ? 2 : 1;
+    known[dev].store(k, std::memory_order_relaxed);
+  }
+  return k == 2;
+}
+static_assert(NB_G1_GRAD_SMALL_TENSORS <= GN_FEW, "a short list is one table");
 
 bool limits_ok(double max_norm, double eps) { return max_norm >= 0 && eps >= 0 && std::isfinite(eps); }
 
@@ -224,14 +267,18 @@ int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, v
 int nb_g1_grad_clip(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
                     const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
                     double max_norm, double eps, void* work, float* norm, long long* bad) {
-  if (!grads_ok(count, grads, sizes, types) || !work || reinterpret_cast<uintptr_t>(work) % 16 ||
-      !limits_ok(max_norm, eps))
-    return (int)cudaErrorInvalidValue;
+  if (!grads_ok(count, grads, sizes, types) || !limits_ok(max_norm, eps)) return (int)cudaErrorInvalidValue;
+  const bool small = grad_small(count, sizes);
+  if (!small && (!work || reinterpret_cast<uintptr_t>(work) % 16)) return (int)cudaErrorInvalidValue;
   if (outs) {
     const int e = outs_error(count, grads, outs, sizes, types, out_types);
     if (e) return e;
   }
   const GradList g = {count, grads, outs, sizes, types, out_types, zero_nonfinite};
+  if (small) {
+    const auto clip = cluster_of_16() ? grad_clip_small<16> : grad_clip_small<8>;
+    return clip(stream, g, max_norm, eps, norm, bad);
+  }
   double2* part = static_cast<double2*>(work);
   int parts = 0;
   const int e = grad_sumsq(stream, g, part, &parts);

@@ -69,7 +69,9 @@ SHAPES = {
     "one value": [(1,)], "one": [(1000,)], "odd": [(1,), (7,), (33, 5), (8191,), (8192,), (8193,), (3, 3, 3)],
     "policy": [(100,), (100,), (128, 100), (128,), (128,), (29, 128), (29,)], "empty ones": [(0,), (5,), (0, 4), (6,)],
     "many": [(k % 37 + 1,) for k in range(500)], "long": [(3_000_001,), (17,), (1_000_000,)],
-    "ctrl": [(8, 4096, 29)],
+    "ctrl": [(8, 4096, 29)], "last of one launch": [(524_287,), (1,)], "first of two": [(524_288,), (1,)],
+    "one table": [(k % 50 + 1,) for k in range(96)], "a tensor more": [(k % 50 + 1,) for k in range(97)],
+    "three tables": [(k % 9 * 100 + 1,) for k in range(2000)],
 }
 
 

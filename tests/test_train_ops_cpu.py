@@ -57,9 +57,11 @@ def test_grad_entries_refuse_bad_arguments():
     lib = capi.load()
     base = 1 << 20
     one = [(base, 10, 0)]
-    for kw in (dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(eps=-1.0), dict(eps=float("nan")),
-               dict(work=NUL)):
+    for kw in (dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(eps=-1.0), dict(eps=float("nan"))):
         assert _clip(one, one, **kw) == INVALID, kw
+    for many in ([(base, 1 << 20, 0)], [(base + 4096 * k, 10, 0) for k in range(97)]):  # (a short list needs no work)
+        for work in (NUL, ctypes.c_void_p((1 << 20) + 8)):
+            assert _clip(many, many, work=work) == INVALID
     for bad in ([(None, 10, 0)], [(base, -1, 0)], [(base, 10, 3)], [(base + 2, 10, 0)], [(base + 1, 10, 1)]):
         assert _clip(bad, bad) == INVALID, bad
         n, g, sizes, types = _arrays(*bad)
