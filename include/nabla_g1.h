@@ -187,8 +187,8 @@ int nb_g1_diag_forward_ex(cudaStream_t stream, unsigned long long* counters, int
  * The backward takes g_y (rows `g_stride` apart, x's type) and the forward's mean and rstd:
  *   h = g_y weight, xh = (x - mean) rstd, g_x = rstd (h - mean(h) - xh mean(h xh)),
  *   g_weight = sum over rows of g_y xh, g_bias = sum over rows of g_y (both of type wtype)
- * g_x, g_weight and g_bias may each be NULL (not wanted); work: nb_g1_layer_norm_work_bytes(rows, cols) bytes, needed
- * for g_weight or g_bias. With no rows g_weight and g_bias are zero. Sums are float32. */
+ * g_x, g_weight and g_bias may each be NULL (not wanted); work: nb_g1_layer_norm_work_bytes(rows, cols) bytes,
+ * 16-byte aligned, needed for g_weight or g_bias. With no rows g_weight and g_bias are zero. Sums are float32. */
 long long nb_g1_layer_norm_work_bytes(long long rows, long long cols);
 int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols, long long stride, int dtype,
                              const void* x, int wtype, const void* weight, const void* bias, float eps, void* y,

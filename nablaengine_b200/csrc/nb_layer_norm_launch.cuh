@@ -46,9 +46,17 @@ inline LnPlan ln_plan(long long rows, int cols, int e, bool backward) {
   const bool split = backward && ln_split_rows(cols);  // (tiles of one row, and more of them)
   p.per_sm = ln_per_sm(lanes, e, backward, p.t.split > 1);
   const long long slots = (long long)SMS * p.per_sm / p.t.split, rounds = (rows + groups - 1) / groups;
-  // a tile of about ln_tile bytes, but not so long that a block has no tile
-  const int per_group = split ? 1 : (int)std::max<long long>(
+  // Tiles of about ln_tile bytes; where a block has few of them, of the length that leaves the busiest block the least
+  // rounds (a tile's own cost: a quarter of one).
+  int per_group = split ? 1 : (int)std::max<long long>(
       1, std::min<long long>(ln_tile(lanes, backward) / (groups * row * tensors), (rounds + slots - 1) / slots));
+  if (rounds < 8 * slots * per_group) {
+    double least = 1e30;
+    for (int k = per_group, longest = k; k >= 1 && k > longest / 2; k--) {
+      const double tiles = (double)(((rounds + k - 1) / k + slots - 1) / slots), cost = tiles * (k + 0.25);
+      if (cost < least) least = cost, per_group = k;
+    }
+  }
   p.t.rows = rows, p.t.cols = cols, p.t.per_tile = groups * per_group;
   p.t.tile_bytes = (p.t.per_tile * row + 15) / 16 * 16 + 16;  // (16: a first row that starts inside a piece)
   p.t.stage_bytes = tensors * p.t.tile_bytes + (backward ? (8 * p.t.per_tile + 15) / 16 * 16 : 0);

@@ -225,7 +225,8 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
   if ((rows && (!g_y || !x || !mean || !rstd)) || !aligned(g_y, dtype) || !aligned(x, dtype) ||
       !aligned(g_x, dtype) || !aligned(weight, wtype) || !aligned(g_weight, wtype) || !aligned(g_bias, wtype))
     return (int)cudaErrorInvalidValue;
-  if (rows && (g_weight || g_bias) && !work) return (int)cudaErrorInvalidValue;
+  if ((g_weight || g_bias) && ((rows && !work) || reinterpret_cast<uintptr_t>(work) % 16))
+    return (int)cudaErrorInvalidValue;
   const LnBackward a = {stream, rows, (int)cols, g_stride, stride, g_y, x, mean, rstd,
                         wtype, weight, g_x, g_weight, g_bias, static_cast<float*>(work)};
   return dtype == F32 ? ln_backward<float>(a) : dtype == BF16 ? ln_backward<__nv_bfloat16>(a)

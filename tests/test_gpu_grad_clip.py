@@ -194,6 +194,20 @@ def test_repeats_bit_for_bit_streams_and_capture():
     _check_outs(outs, _reference(grads, 1.0, 1e-6, False)[2])
 
 
+def test_offsets_beyond_32_bits():
+    torch = _torch()
+    from nablaengine_b200 import torch_ffi
+    g = torch.zeros(2 ** 31 + 4099, dtype=torch.bfloat16, device="cuda")
+    at = [0, 7, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 4098]
+    g[at] = torch.tensor([3.0, -4.0, 12.0, 84.0, 3612.0], dtype=torch.bfloat16, device="cuda")
+    exact = math.sqrt(sum(float(v) ** 2 for v in g[at]))
+    before = g[at].double()
+    norm, bad = torch_ffi.clip_grad_norm([g], 1.0)
+    assert abs(float(norm) - exact) <= 5 * U * exact and int(bad) == 0
+    _check_outs([g[at]], [before / (exact + 1e-6)])
+    assert int((g != 0).sum()) == len(at)
+
+
 def test_in_place_is_seen_by_autograd():
     torch = _torch()
     from nablaengine_b200 import torch_ffi

@@ -202,6 +202,46 @@ def test_nan_and_inf_stay_in_their_rows():
         assert torch.isnan(gw).all() and torch.isfinite(gb).all()
 
 
+@pytest.mark.parametrize("cols", [6001, 8192, 12000, 20001, 40000])
+def test_nan_stays_in_its_row_where_a_row_takes_many_warps(cols):
+    torch = _torch()
+    from nablaengine_b200 import torch_ffi
+    x, w, b, gy = _inputs(9, cols, torch.bfloat16, "f32")
+    clean = torch_ffi.layer_norm_forward(x, w, b)
+    cg = torch_ffi.layer_norm_backward(gy, x, clean[1], clean[2], w, b)[0]
+    x[4, cols // 2] = float("nan")
+    y, mean, rstd = torch_ffi.layer_norm_forward(x, w, b)
+    gx = torch_ffi.layer_norm_backward(gy, x, mean, rstd, w, b)[0]
+    rest = [0, 1, 2, 3, 5, 6, 7, 8]
+    assert torch.equal(y[rest], clean[0][rest]) and torch.equal(gx[rest], cg[rest])
+    assert torch.isnan(y[4]).all() and torch.isnan(gx[4]).all()
+
+
+@pytest.mark.parametrize("cols", [512, 1001])
+def test_offsets_beyond_32_bits(cols):
+    """More than 2^31 values: the last rows equal those rows alone, bit for bit (a row does not depend on the others),
+    and the column sums the sums of the halves' (to the rounding of sums of random signs)."""
+    torch = _torch()
+    from nablaengine_b200 import torch_ffi
+    rows = 2 ** 31 // cols + 1000
+    part = (torch.randn(1 << 16, cols, device="cuda") * 2 + 1).to(torch.bfloat16)
+    x = part.repeat(rows // (1 << 16) + 1, 1)[:rows]
+    g = x.flip(1) if cols % 2 else x
+    w, b = torch.rand(cols, device="cuda"), torch.rand(cols, device="cuda")
+    y, mean, rstd = torch_ffi.layer_norm_forward(x, w, b)
+    gx, gw, gb = torch_ffi.layer_norm_backward(g, x, mean, rstd, w, b)
+    tail = slice(rows - 777, rows)
+    ty, tm, tr = torch_ffi.layer_norm_forward(x[tail].clone(), w, b)
+    tgx = torch_ffi.layer_norm_backward(g[tail].clone(), x[tail].clone(), tm, tr, w, b)[0]
+    assert torch.equal(y[tail], ty) and torch.equal(mean[tail], tm) and torch.equal(rstd[tail], tr)
+    assert torch.equal(gx[tail], tgx)
+    half = rows // 2
+    parts = [torch_ffi.layer_norm_backward(g[s].clone(), x[s].clone(), mean[s].clone(), rstd[s].clone(), w, b)
+             for s in (slice(0, half), slice(half, rows))]
+    for whole, a, c in zip((gw, gb), parts[0][1:], parts[1][1:]):
+        assert ((whole - (a + c)).abs() <= 1e-4 * (a.abs() + c.abs()) + 1e-2).all()
+
+
 def test_no_rows():
     torch = _torch()
     from nablaengine_b200 import torch_ffi

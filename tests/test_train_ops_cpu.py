@@ -34,7 +34,7 @@ def test_layer_norm_entries_refuse_bad_arguments():
         assert forward(**kw) == INVALID, kw
     for kw in (dict(rows=-1), dict(cols=0), dict(gs=-1), dict(s=-1), dict(dtype=7), dict(dtype=2, wtype=1),
                dict(g=NUL), dict(x=NUL), dict(mean=NUL), dict(rstd=NUL), dict(work=NUL), dict(gx=odd), dict(g=odd),
-               dict(gw=odd)):
+               dict(gw=odd), dict(work=ctypes.c_void_p((1 << 20) + 8))):
         assert backward(**kw) == INVALID, kw
     assert lib.nb_g1_layer_norm_work_bytes(4096, 100) > 0
     assert lib.nb_g1_layer_norm_work_bytes(-1, 100) < 0 and lib.nb_g1_layer_norm_work_bytes(1, 0) < 0
