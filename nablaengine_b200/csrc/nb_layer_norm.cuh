@@ -250,7 +250,6 @@ __device__ __forceinline__ void store_row(T* row, int cols, int lane, const floa
   }
 }
 
-// Set the places beyond the last column to 0.
 // A thread's float32 values at its columns of `row` (any alignment of its start where V is 1 or 2).
 template <int LANES, int EPT, int V, bool FULL>
 __device__ __forceinline__ void store_sums(float* row, int cols, int lane, const float2* v) {
@@ -268,11 +267,16 @@ __device__ __forceinline__ void store_sums(float* row, int cols, int lane, const
   }
 }
 
+// Set the places beyond the last column to 0 (a vector is on one side of it).
 template <int LANES, int EPT, int V>
 __device__ __forceinline__ void clear_beyond(int cols, int lane, float2* v) {
 #pragma unroll
-  for (int i = 0; i < EPT; i++)
-    if (ln_column<LANES, V>(lane, i) >= cols) (i % 2 ? v[i / 2].y : v[i / 2].x) = 0.f;
+  for (int j = 0; j < EPT / V; j++) {
+    const bool beyond = (j * LANES + lane) * V >= cols;
+#pragma unroll
+    for (int k = j * V; k < (j + 1) * V; k++)
+      if (beyond) (k % 2 ? v[k / 2].y : v[k / 2].x) = 0.f;
+  }
 }
 
 // FULL: every block has LANES * EPT columns (no thread has a place beyond the last); SPLIT: a row is split over the
