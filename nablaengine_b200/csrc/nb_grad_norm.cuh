@@ -10,7 +10,9 @@
 //
 // Both passes are bound by memory. The tensors are cut into chunks that the blocks take in turn, in the first pass from
 // the first chunk on and in the second from the last one back, so that the second finds in the second-level cache
-// what the first read last.
+// what the first read last (30.4M float32 values: 22 us, 5.5 TB/s, and 34 us, of which 70 MB come from the cache; the
+// second pass is bound by what it writes, 3.5 TB/s, as much as a plain copy writes: keeping 28 MB more on the chip
+// changed nothing). 100M bfloat16 values: 98 us.
 #pragma once
 #include <cstdint>
 #include "nb_values.cuh"

@@ -9,6 +9,12 @@
 // From shared memory a row goes to the registers of `lanes` threads (8 to 1024, a power of two), EPT values each. A
 // thread keeps the same columns for every row it takes, so the weight, the bias and the two column sums of the backward
 // stay in its registers too. Rows that do not fit take the row-in-memory kernels at the end.
+//
+// Memory bounds both directions (8 and 14 operations a value). 131072 x 512: forward bfloat16 50 us, 5.4 TB/s; backward
+// float32 139 us, 5.8 TB/s with the sum of the column sums (a plain copy reaches 6.55). 16-bit rows of an odd width are
+// bound by their instructions (values one by one: 65536 x 1001 float16 forward 71 us, backward 121), and the backward
+// of rows of more than 4096 columns by one block an SM, whose 16 warps meet at each row (8192 x 8192 bfloat16: 86 us,
+// 4.7 TB/s).
 #pragma once
 #include <cstdint>
 #include "nb_values.cuh"
@@ -279,8 +285,9 @@ __device__ __forceinline__ void clear_beyond(int cols, int lane, float2* v) {
   }
 }
 
-// FULL: every block has LANES * EPT columns (no thread has a place beyond the last); SPLIT: a row is split over the
-// blocks of a cluster
+// The forward: the row's mean, then the variance from the deviations in registers, each sum over the lanes; rstd by
+// rsqrtf (2 units in the last place at most, below what the variance's sum leaves). FULL: every block has LANES * EPT
+// columns (no thread has a place beyond the last); SPLIT: a row is split over the blocks of a cluster.
 template <class T, int LANES, int EPT, int V, bool FULL, bool SPLIT>
 __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm(LANES, sizeof(T), false, SPLIT))
     k_ln_forward(LnTiles t, int kind, long long stride, const T* __restrict__ x, int wtype,
@@ -357,7 +364,9 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
   if (SPLIT) cluster_barrier();  // (nobody leaves while others put sums into its slots)
 }
 
-// part (gridDim.x, 2, cols), if wanted: the block's column sums of g xh and g
+// The backward: both sums of a row (h and h xh) meet in one exchange; (x - mean) rstd is taken as written, not as one
+// fused product, which would leave rounding where x is the mean. part (gridDim.x, 2, cols), if wanted: the block's
+// column sums of g xh and g, which k_ln_backward_sum adds up in a fixed order.
 template <class T, int LANES, int EPT, int V, bool FULL>
 __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(LANES, sizeof(T), true, false))
     k_ln_backward(LnTiles t, int gkind, long long gstride, int kind, long long stride, const T* __restrict__ gy,
