@@ -6,7 +6,7 @@
 // A block takes tiles of rows in turn. The tiles come through a ring of up to four stages in shared memory, filled by
 // asynchronous copies, so loads are in flight while a tile is worked on, and a dense x is copied in 16-byte pieces
 // whatever its width: a tile is one span of memory, rounded out to whole pieces, and a row starts where it starts.
-// From shared memory a row goes to the registers of `lanes` threads (8 to 1024, a power of two), EPT values each. A
+// From shared memory a row goes to the registers of `lanes` threads (8 to 512, a power of two), EPT values each. A
 // thread keeps the same columns for every row it takes, so the weight, the bias and the two column sums of the backward
 // stay in its registers too. Rows that do not fit take the row-in-memory kernels at the end.
 //
@@ -599,29 +599,44 @@ __global__ void __launch_bounds__(LANES, 512 / LANES)
   store_sums<LANES, EPT, V, FULL>(sums + t.cols, cols, lane, gb);
 }
 
-// gw, gb = the sums of the blocks' column sums: 32 columns a block, a warp for each WARPS-th of the parts
-template <class W, int WARPS>
+// gw, gb = the sums of the blocks' column sums: 32 V columns a block, a warp for each WARPS-th of the parts
+template <class W, int WARPS, int V>
 __global__ void __launch_bounds__(32 * WARPS) k_ln_backward_sum(int parts, int cols, const float* __restrict__ part,
                                                                 W* __restrict__ gw, W* __restrict__ gb) {
-  __shared__ float s[WARPS][32];
+  __shared__ float s[WARPS][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;  // 0 .. 2 cols: gw's columns, then gb's
+  const int c = (blockIdx.x * 32 + lane) * V;  // 0 .. 2 cols: gw's columns, then gb's (V divides both)
   let_next_start();
   wait_for_last();
-  float v = 0.f;
+  float v[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) v[k] = 0.f;
   if (c < 2 * cols) {
 #pragma unroll 10
-    for (int p = warp; p < parts; p += WARPS) v += part[(long long)p * 2 * cols + c];
+    for (int p = warp; p < parts; p += WARPS) {
+      const float* from = part + (long long)p * 2 * cols + c;
+      if constexpr (V == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(from);
+        v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
+      } else {
+        v[0] += *from;
+      }
+    }
   }
-  s[warp][lane] = v;
-  __syncthreads();
-  if (warp || c >= 2 * cols) return;
 #pragma unroll
-  for (int k = 1; k < WARPS; k++) v += s[k][lane];
-  if (c < cols) {
-    if (gw) gw[c] = from_f32<W>(v);
-  } else if (gb) {
-    gb[c - cols] = from_f32<W>(v);
+  for (int k = 0; k < V; k++) s[warp][lane * V + k] = v[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 32 * WARPS) {
+    const int at = blockIdx.x * 32 * V + i;
+    if (at >= 2 * cols) continue;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; k++) t += s[k][i];
+    if (at < cols) {
+      if (gw) gw[at] = from_f32<W>(t);
+    } else if (gb) {
+      gb[at - cols] = from_f32<W>(t);
+    }
   }
 }
 

@@ -235,12 +235,15 @@ template <class T> int ln_backward(const LnBackward& a) {
   if (e || !sums) return e;
   ln_param_type<T>(a.wtype, [&](auto w) {
     using W = decltype(w);
-    // (many warps to a column where there are few columns, few where a block would wait for its place)
-    auto sum = [&](auto warps) {
-      return launch_after({a.stream, (2 * a.cols + 31) / 32, 32 * warps.value}, k_ln_backward_sum<W, warps.value>,
-                          parts, a.cols, a.part, static_cast<W*>(a.gw), static_cast<W*>(a.gb));
+    // four columns to a thread where there are many (8192 x 8192 bfloat16 in all 80.6 us, 82.3 with one, 77.1 without
+    // the sum)
+    auto sum = [&](auto warps, auto v) {
+      constexpr int WIDE = 32 * v.value;
+      return launch_after({a.stream, (2 * a.cols + WIDE - 1) / WIDE, 32 * warps.value},
+                          k_ln_backward_sum<W, warps.value, v.value>, parts, a.cols, a.part, static_cast<W*>(a.gw),
+                          static_cast<W*>(a.gb));
     };
-    e = a.cols <= 2048 ? sum(Int<32>()) : sum(Int<8>());
+    e = a.cols <= 2048 ? sum(Int<32>(), Int<1>()) : a.cols % 4 ? sum(Int<8>(), Int<1>()) : sum(Int<32>(), Int<4>());
   });
   return e;
 }
