@@ -12,9 +12,10 @@ namespace nbtrain {
 
 // How a layer norm of rows that a ring holds is spread: the tiles, and the blocks (clusters) that take them in turn.
 constexpr int LN_SMEM = 224 * 1024, LN_SMEM_SM = 220 * 1024;
-// bytes of a tile, of all tensors (131072 x 512 float32 backward: 128 us with 32 KB, 146 with 64; 8192 x 8192 bfloat16,
-// whose one block an SM waits at each tile: 88 us with 64, 97 with 32)
-constexpr int ln_tile(int lanes, bool backward) { return !backward ? 49152 : lanes > LN_LANES ? 65536 : 32768; }
+// bytes of a tile, of all tensors and the backward's two floats a row: 48 KB of rows, or 64, and room for the floats
+// (backward, bfloat16 131072 x 512: 70 us with 48 KB, 76 with 32; 8192 x 8192, whose one block an SM waits at each
+// tile: 81 us with 64 KB, 93 with 32)
+constexpr int ln_tile(int lanes) { return lanes > LN_LANES ? 67 * 1024 : 50 * 1024; }
 struct LnPlan {
   LnTiles t;
   int blocks, smem, per_sm;
@@ -48,8 +49,10 @@ inline LnPlan ln_plan(long long rows, int cols, int e, bool backward) {
   const long long slots = (long long)SMS * p.per_sm / p.t.split, rounds = (rows + groups - 1) / groups;
   // Tiles of about ln_tile bytes; where a block has few of them, of the length that leaves the busiest block the least
   // rounds (a tile's own cost: a quarter of one).
-  int per_group = split ? 1 : (int)std::max<long long>(
-      1, std::min<long long>(ln_tile(lanes, backward) / (groups * row * tensors), (rounds + slots - 1) / slots));
+  const int round = groups * (row * tensors + (backward ? 8 : 0));
+  int per_group = 1;
+  if (!split)
+    per_group = (int)std::max<long long>(1, std::min<long long>(ln_tile(lanes) / round, (rounds + slots - 1) / slots));
   if (rounds < 8 * slots * per_group) {
     double least = 1e30;
     for (int k = per_group, longest = k; k >= 1 && k > longest / 2; k--) {

@@ -119,11 +119,13 @@ def _both(x, w, b, gy, eps=1e-5):
 # registers and beyond its shared memory), row counts that fill no block and that fill many waves
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,cols", [
-    (1, 1), (3, 1), (1, 2), (5, 7), (2, 8), (1, 31), (9, 32), (4, 33), (17, 35), (33, 36), (64, 64), (257, 71), (100, 99),
-    (4096, 100), (129, 127), (31, 128), (7, 129), (130, 255), (61, 256), (40, 257), (300, 512), (45, 513), (77, 1000),
-    (50, 1001), (20, 1024), (19, 2047), (301, 2048), (6, 4096), (151, 4100), (3, 8191), (160, 8192), (2, 16384),
+    (1, 1), (3, 1), (1, 2), (5, 7), (2, 8), (1, 31), (9, 32), (4, 33), (17, 35), (33, 36), (64, 64), (257, 71),
+    (100, 99), (4096, 100), (129, 127), (31, 128), (7, 129), (130, 255), (61, 256), (40, 257), (300, 512), (45, 513),
+    (77, 1000), (50, 1001), (20, 1024), (19, 2047), (301, 2048), (6, 4096), (151, 4100), (3, 8191), (160, 8192),
+    (2, 16384),
     (2, 16385), (1, 40000), (3, 65537), (1, 300001), (100003, 5), (500, 8192), (331, 8208), (97, 9001), (700, 12000),
-    (333, 16384), (40, 20001), (350, 32768), (5, 32769), (3001, 64), (77, 63), (20011, 3)])
+    (333, 16384), (40, 20001), (350, 32768), (5, 32769), (3001, 64), (77, 63), (20011, 3),
+    (70001, 1), (300_000, 2), (40_000, 9)])
 def test_sizes_and_types(rows, cols, dtype):
     x, w, b, gy = _inputs(rows, cols, _dtype(dtype), "f32", seed=rows + cols)
     _both(x, w, b, gy)
