@@ -12,9 +12,9 @@
 //
 // Memory bounds both directions (8 and 14 operations a value). 131072 x 512: forward bfloat16 50 us, 5.4 TB/s; backward
 // float32 139 us, 5.8 TB/s with the sum of the column sums (a plain copy reaches 6.55). 16-bit rows of an odd width are
-// bound by their instructions (values one by one: 65536 x 1001 float16 forward 71 us, backward 121), and the backward
-// of rows of more than 4096 columns by one block an SM, whose 16 warps meet at each row (8192 x 8192 bfloat16: 86 us,
-// 4.7 TB/s).
+// bound by their instructions (values one by one: 65536 x 1001 float16 forward 71 us, backward 113), and the backward
+// of rows of more than 4096 columns by one block an SM, whose 16 warps meet at each row (8192 x 8192 bfloat16: 83 us,
+// 4.8 TB/s).
 #pragma once
 #include <cstdint>
 #include "nb_values.cuh"
@@ -334,8 +334,9 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
     const T* rows = reinterpret_cast<const T*>(ring + stage * t.stage_bytes + feed.phase(at));
     free_stage = stage;
     stage = stage + 1 == t.stages ? 0 : stage + 1;
-    // (two rows' loops in one where it gains: 65536 x 1024 bfloat16 47.8 -> 45.6 us; 131072 x 512 float32 85 -> 90)
-    constexpr int TOGETHER = sizeof(T) == 2 && LANES > 32 ? 2 : 1;
+    // (two rows' loops in one where it gains: 65536 x 1024 bfloat16 47.8 -> 45.6 us; not 131072 x 512 float32, 85 ->
+    // 90, nor 65536 x 1001 bfloat16, 71 -> 80)
+    constexpr int TOGETHER = sizeof(T) == 2 && LANES > 32 && V > 1 ? 2 : 1;
 #pragma unroll TOGETHER
     for (int r0 = g.index - shift; r0 < n; r0 += GROUPS) {  // (r0: the warp's first row)
       const int r = r0 + shift;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
 // t.width columns to a block. The two sums of a row meet in the slots of all its blocks
 // under the cluster's barrier, which is split: between arriving with row k's sums and waiting for the others' a thread
 // finishes row k - 1, from shared memory again: nobody stands still for the exchange, for half as many instructions
-// again (8192 x 8192 bfloat16, which needs no cluster, takes 103 us here and 94 in k_ln_backward). part (teams, 2,
+// again (8192 x 8192 bfloat16, which needs no cluster, took 103 us here when k_ln_backward took 94). part (teams, 2,
 // cols), if wanted.
 template <class T, int LANES, int V, bool FULL>
 __global__ void __launch_bounds__(LANES, 512 / LANES)
