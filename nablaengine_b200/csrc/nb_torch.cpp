@@ -57,11 +57,13 @@ int code_of(const Tensor& t) {
   }
 }
 
-// A tensor argument: its tensor if it is one on a GPU of a value type, else null.
+// A tensor argument: its tensor if it is one on a GPU of a value type whose memory holds its values (no lazy negation),
+// else null.
 const Tensor* gpu_tensor(PyObject* x) {
   if (!THPVariable_Check(x)) return nullptr;
   const Tensor& t = THPVariable_Unpack(x);
-  return t.is_cuda() && t.layout() == at::kStrided && code_of(t) >= 0 ? &t : nullptr;
+  const bool plain = t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !t._is_zerotensor();
+  return plain && code_of(t) >= 0 ? &t : nullptr;
 }
 
 int gpu_of(const Tensor& t) { return t.get_device(); }

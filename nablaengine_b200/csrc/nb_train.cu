@@ -24,12 +24,16 @@ bool ln_args_ok(long long rows, long long cols, long long stride, int dtype, int
 bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) == 0; }
 
 // ---- the gradient list ----------------------------------------------------------------------------------------------
+constexpr long long GRAD_LONGEST = 1ll << 40;  // values of a tensor: more than any GPU holds
+
 bool grads_ok(int count, const void* const* in, const long long* sizes, const int* types) {
   if (count < 0) return false;
   if (count == 0) return true;
   if (!in || !sizes || !types) return false;
   for (int i = 0; i < count; i++)
-    if (sizes[i] < 0 || !dtype_ok(types[i]) || (sizes[i] && (!in[i] || !aligned(in[i], types[i])))) return false;
+    if (sizes[i] < 0 || sizes[i] > GRAD_LONGEST || !dtype_ok(types[i]) ||
+        (sizes[i] && (!in[i] || !aligned(in[i], types[i]))))
+      return false;
   return true;
 }
 
@@ -194,6 +198,9 @@ bool cluster_of_16() {
 static_assert(NB_G1_GRAD_SMALL_TENSORS <= GN_FEW, "a short list is one table");
 
 bool limits_ok(double max_norm, double eps) { return max_norm >= 0 && eps >= 0 && std::isfinite(eps); }
+bool results_ok(const float* norm, const long long* bad) {
+  return aligned(norm, F32) && reinterpret_cast<uintptr_t>(bad) % 8 == 0;
+}
 
 }  // namespace
 
@@ -211,7 +218,7 @@ int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols
     return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   if (!x || !y || !mean || !rstd || !aligned(x, dtype) || !aligned(y, dtype) || !aligned(weight, wtype) ||
-      !aligned(bias, wtype))
+      !aligned(bias, wtype) || !aligned(mean, F32) || !aligned(rstd, F32))
     return (int)cudaErrorInvalidValue;
   const LnForward a = {stream, rows, (int)cols, stride, x, wtype, weight, bias, eps, y, mean, rstd};
   return dtype == F32 ? ln_forward<float>(a) : dtype == BF16 ? ln_forward<__nv_bfloat16>(a) : ln_forward<__half>(a);
@@ -223,7 +230,8 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
                               void* g_bias, void* work) {
   if (!ln_args_ok(rows, cols, stride, dtype, wtype) || g_stride < 0) return (int)cudaErrorInvalidValue;
   if ((rows && (!g_y || !x || !mean || !rstd)) || !aligned(g_y, dtype) || !aligned(x, dtype) ||
-      !aligned(g_x, dtype) || !aligned(weight, wtype) || !aligned(g_weight, wtype) || !aligned(g_bias, wtype))
+      !aligned(g_x, dtype) || !aligned(weight, wtype) || !aligned(g_weight, wtype) || !aligned(g_bias, wtype) ||
+      !aligned(mean, F32) || !aligned(rstd, F32))
     return (int)cudaErrorInvalidValue;
   if ((g_weight || g_bias) && ((rows && !work) || reinterpret_cast<uintptr_t>(work) % 16))
     return (int)cudaErrorInvalidValue;
@@ -255,7 +263,7 @@ int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, v
                      const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
                      double max_norm, double eps, const double* stats, float* norm, long long* bad) {
   if (!grads_ok(count, grads, sizes, types) || !stats || reinterpret_cast<uintptr_t>(stats) % 16 ||
-      !limits_ok(max_norm, eps))
+      !limits_ok(max_norm, eps) || !results_ok(norm, bad))
     return (int)cudaErrorInvalidValue;
   if (outs) {
     const int e = outs_error(count, grads, outs, sizes, types, out_types);
@@ -268,7 +276,8 @@ int nb_g1_grad_scale(cudaStream_t stream, int count, const void* const* grads, v
 int nb_g1_grad_clip(cudaStream_t stream, int count, const void* const* grads, void* const* outs,
                     const long long* sizes, const int* types, const int* out_types, int zero_nonfinite,
                     double max_norm, double eps, void* work, float* norm, long long* bad) {
-  if (!grads_ok(count, grads, sizes, types) || !limits_ok(max_norm, eps)) return (int)cudaErrorInvalidValue;
+  if (!grads_ok(count, grads, sizes, types) || !limits_ok(max_norm, eps) || !results_ok(norm, bad))
+    return (int)cudaErrorInvalidValue;
   const bool small = grad_small(count, sizes);
   if (!small && (!work || reinterpret_cast<uintptr_t>(work) % 16)) return (int)cudaErrorInvalidValue;
   if (outs) {

@@ -231,7 +231,8 @@ def test_refusals():
     torch = _torch()
     from nablaengine_b200 import torch_ffi
     g = torch.randn(64, 8, device="cuda")
-    for bad in (g, [g.cpu()], [g.double()], [g[:, ::2]], [g.expand(3, 64, 8)], [None], [g, g.int()], [g[::2]]):
+    for bad in (g, [g.cpu()], [g.double()], [g[:, ::2]], [g.expand(3, 64, 8)], [None], [g, g.int()], [g[::2]],
+                [torch._neg_view(g)]):
         with pytest.raises(TypeError):
             torch_ffi.grad_norm(bad)
         with pytest.raises(TypeError):

@@ -364,7 +364,7 @@ def test_refusals():
     x, w, b, gy = _inputs(8, 36, torch.float32, "f32")
     y, mean, rstd = torch_ffi.layer_norm_forward(x, w, b)
     for bad in (x.cpu(), x.double(), x.t(), x[:, ::2], torch.zeros((), device="cuda"), torch.zeros(4, 0, device="cuda"),
-                x.view(2, 4, 36)[:, ::3].transpose(0, 1), None):
+                x.view(2, 4, 36)[:, ::3].transpose(0, 1), None, torch._neg_view(x)):
         with pytest.raises(TypeError):
             torch_ffi.layer_norm(bad)
     for bad in (w[:35], w.cpu(), w.double(), w.half(), torch.ones(72, device="cuda")[::2], w.view(1, 36)):

@@ -30,11 +30,11 @@ def test_layer_norm_entries_refuse_bad_arguments():
     for kw in (dict(rows=-1), dict(cols=0), dict(cols=-3), dict(cols=1 << 40), dict(stride=-1), dict(dtype=3),
                dict(dtype=-1), dict(dtype=0, wtype=1), dict(dtype=1, wtype=2), dict(x=NUL), dict(y=NUL),
                dict(mean=NUL), dict(rstd=NUL), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")),
-               dict(x=odd), dict(y=odd), dict(w=odd), dict(b=odd)):
+               dict(x=odd), dict(y=odd), dict(w=odd), dict(b=odd), dict(mean=odd), dict(rstd=odd)):
         assert forward(**kw) == INVALID, kw
     for kw in (dict(rows=-1), dict(cols=0), dict(gs=-1), dict(s=-1), dict(dtype=7), dict(dtype=2, wtype=1),
                dict(g=NUL), dict(x=NUL), dict(mean=NUL), dict(rstd=NUL), dict(work=NUL), dict(gx=odd), dict(g=odd),
-               dict(gw=odd), dict(work=ctypes.c_void_p((1 << 20) + 8))):
+               dict(gw=odd), dict(mean=odd), dict(rstd=odd), dict(work=ctypes.c_void_p((1 << 20) + 8))):
         assert backward(**kw) == INVALID, kw
     assert lib.nb_g1_layer_norm_work_bytes(4096, 100) > 0
     assert lib.nb_g1_layer_norm_work_bytes(-1, 100) < 0 and lib.nb_g1_layer_norm_work_bytes(1, 0) < 0
@@ -70,6 +70,18 @@ def test_grad_entries_refuse_bad_arguments():
     assert lib.nb_g1_grad_sumsq(NUL, -1, NUL, NUL, NUL, 0, AT, AT) == INVALID
     assert lib.nb_g1_grad_work_bytes(-1) < 0 and lib.nb_g1_grad_work_bytes(0) > 0
     assert lib.nb_g1_grad_work_bytes(1000) >= lib.nb_g1_grad_work_bytes(10)
+
+
+def test_grad_results_refuse_odd_addresses_and_impossible_sizes():
+    lib = capi.load()
+    base = 1 << 20
+    n, g, sizes, types = _arrays((base, 10, 0))
+    for norm, bad in ((base + 2, base), (base, base + 4)):
+        at = ctypes.c_void_p(norm), ctypes.c_void_p(bad)
+        assert lib.nb_g1_grad_clip(NUL, n, g, g, sizes, types, types, 0, 1.0, 0.0, AT, *at) == INVALID
+        assert lib.nb_g1_grad_scale(NUL, n, g, g, sizes, types, types, 0, 1.0, 0.0, AT, *at) == INVALID
+    for size in ((1 << 40) + 1, (1 << 63) - 1):
+        assert _clip([(base, size, 0)], [(base, size, 0)]) == INVALID
 
 
 def test_grad_entries_refuse_shared_memory():
