@@ -99,3 +99,35 @@ def check_backward(gy, x, mean, rstd, w, b, gx, gw, gb):
     if b is not None:
         assert gb.dtype == b.dtype and gb.shape == (n,)
         within("g_bias", gb, rb, kr * U * g2.abs().sum(0) + half_ulp(rb, b.dtype))
+
+
+def exact_sums_inputs(rows, cols, dtype, seed=0, device="cuda"):
+    """(g_y, x, mean, rstd) whose column sums float32 holds exactly in any order: g_y is 1 or -1 everywhere, so that every
+    row counts in every column, and (x - mean) rstd is a whole number of at most 3 (3 rows < 2^24)."""
+    assert 3 * rows < 2 ** 24
+    g = torch.Generator(device=device).manual_seed(seed)
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, dtype=torch.int8, device=device, generator=g)
+
+    gy = whole(0, 1, rows, cols).mul_(2).sub_(1).to(DTYPES[dtype])
+    x = whole(-2, 2, rows, cols).to(DTYPES[dtype])
+    return gy, x, whole(0, 1, rows).float(), torch.ones(rows, device=device)
+
+
+def check_exact_sums(gy, x, mean, rstd, gw, gb):
+    """g_weight and g_bias of exact_sums_inputs, to the last bit: a row left out, taken twice or read from another place
+    shows."""
+    rows = x.shape[0]
+    want = torch.zeros((2, x.shape[1]), dtype=torch.int64, device=x.device)
+    step = max(1, (1 << 25) // x.shape[1])
+    for r in range(0, rows, step):
+        s = slice(r, min(r + step, rows))
+        g = gy[s].to(torch.int8)
+        xh = ((x[s].float() - mean[s, None]) * rstd[s, None]).to(torch.int8)
+        want[0] += (g * xh).sum(0, dtype=torch.int64)
+        want[1] += g.sum(0, dtype=torch.int64)
+    for name, got, sums in (("g_weight", gw, want[0]), ("g_bias", gb, want[1])):
+        assert got.dtype == torch.float32 and got.shape == sums.shape
+        wrong = got.double() != sums.double()
+        assert not wrong.any(), f"{name}: {int(wrong.sum())} of {wrong.numel()} columns"

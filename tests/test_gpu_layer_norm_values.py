@@ -74,3 +74,27 @@ def test_offsets_scales_and_rows_of_one_value():
     x[3], x[7] = 0.0, -17.25
     for other in (x, x + 1.0e4, x * 1.0e-18, x * 1.0e15):
         _check(other, w, b, gy)
+
+
+def _check_sums(rows, cols, dtype):
+    torch = _torch()
+    from nablaengine_b200 import torch_ffi
+    gy, x, mean, rstd = checks.exact_sums_inputs(rows, cols, dtype, seed=rows + cols)
+    one = torch.ones(cols, device="cuda")
+    _, gw, gb = torch_ffi.layer_norm_backward(gy, x, mean, rstd, one, one)
+    checks.check_exact_sums(gy, x, mean, rstd, gw, gb)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [
+    (1, 100), (2, 33), (100003, 5), (300_000, 2), (70001, 1), (40_000, 9), (262_143, 64), (131_073, 100), (20011, 3),
+    (5000, 1001), (4099, 512), (1023, 4100), (301, 8192), (333, 8208), (777, 12000), (333, 16384), (350, 32768),
+    (70, 32769), (129, 40001)])
+def test_column_sums_take_every_row_once(rows, cols, dtype):
+    _check_sums(rows, cols, dtype)
+
+
+@pytest.mark.parametrize("cols", [512, 1001])
+def test_column_sums_take_every_row_beyond_32_bits(cols):
+    """More than 2^31 values, and rows on either side of that offset."""
+    _check_sums(2 ** 31 // cols + 1000, cols, "bf16")

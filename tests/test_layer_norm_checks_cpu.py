@@ -35,3 +35,20 @@ def test_a_wrong_value_fails(which, whole, value):
         wrong[which].view(-1)[at] = value
         with pytest.raises(AssertionError):
             check(wrong)
+
+
+@pytest.mark.parametrize("rows,cols", [(1000, 7), (100003, 5)])
+def test_column_sums_that_miss_one_row_fail(rows, cols):
+    """The sums of all rows pass; those without one row, with one row twice, or with a NaN do not."""
+    gy, x, mean, rstd = checks.exact_sums_inputs(rows, cols, "f32", device="cpu")
+    terms = gy * (x - mean[:, None]) * rstd[:, None]
+    gw, gb = terms.sum(0, dtype=torch.float64).float(), gy.sum(0, dtype=torch.float64).float()
+    checks.check_exact_sums(gy, x, mean, rstd, gw, gb)
+    for row in (0, rows // 2, rows - 1):
+        for sign in (-1, 1):
+            with pytest.raises(AssertionError):
+                checks.check_exact_sums(gy, x, mean, rstd, gw, gb + sign * gy[row])
+            with pytest.raises(AssertionError):
+                checks.check_exact_sums(gy, x, mean, rstd, gw + sign * (terms[row] + terms[row - 1]) + gy[row], gb)
+    with pytest.raises(AssertionError):
+        checks.check_exact_sums(gy, x, mean, rstd, gw * float("nan"), gb)
