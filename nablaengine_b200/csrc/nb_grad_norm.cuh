@@ -177,9 +177,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_grad_finish(int parts, const dou
   if (bad) *bad = (long long)v.y;
 }
 
-__device__ __forceinline__ float clip_coefficient(double sumsq, double max_norm, double eps) {
+__device__ __forceinline__ double clip_coefficient(double sumsq, double max_norm, double eps) {
   const double d = sqrt(sumsq) + eps;
-  return d <= max_norm ? 1.f : (float)(max_norm / d);  // (a NaN norm gives NaN, an infinite one 0)
+  return d <= max_norm ? 1.0 : max_norm / d;  // (a NaN norm gives NaN, an infinite one 0)
 }
 
 // c v; where non-finite values count as 0 and there are any, those are 0
@@ -201,17 +201,24 @@ template <class O, int P> __device__ __forceinline__ void store_piece(O* p, cons
 }
 
 template <int THREADS, class T, class O>
-__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, int tid, float coef, bool clean) {
+__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, int tid, double exact, bool clean) {
+  // The coefficient is rounded to float32 (as exact as the products' own rounding) unless that is below float32's normal
+  // range, where it has few bits left: then the values are scaled one by one in 64 bits.
+  const float coef = (float)exact;
+  const bool tiny = exact > 0.0 && exact < 0x1p-126;
   constexpr int P = 16 / sizeof(T), STEP = THREADS * GN_UNROLL;
   const T* base = static_cast<const T*>(e.in);
   O* out = static_cast<O*>(e.out);
-  auto one = [&](long long i) { out[i] = from_f32<O>(clip_value(to_f32(base[i]), coef, clean)); };
+  auto one = [&](long long i) {
+    const float v = to_f32(base[i]);
+    out[i] = from_f32<O>(tiny && isfinite(v) ? (float)((double)v * exact) : clip_value(v, coef, clean));
+  };
   if (part.first == e.lead)
     for (int i = tid; i < min((long long)e.lead, e.n); i += THREADS) one(i);
   if (part.n <= 0) return;
   const uint4* from = reinterpret_cast<const uint4*>(base + part.first);
   O* to = out + part.first;
-  const int pieces = e.vectors ? part.n / P : 0;
+  const int pieces = e.vectors && !tiny ? part.n / P : 0;
   auto piece = [&](int at, uint4 u) {
     float2 v[P / 2];
     unpack_piece<T>(u, v);
@@ -235,14 +242,14 @@ __device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, in
 }
 
 template <int THREADS, class T>
-__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, int tid, float coef, bool clean) {
+__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, int tid, double coef, bool clean) {
   if (e.out_type == F32) scale_part<THREADS, T, float>(e, part, tid, coef, clean);
   else if (e.out_type == BF16) scale_part<THREADS, T, __nv_bfloat16>(e, part, tid, coef, clean);
   else scale_part<THREADS, T, __half>(e, part, tid, coef, clean);
 }
 template <int THREADS>
-__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, int tid, float coef, bool clean) {
-  if (coef == 1.f && !clean && e.in == e.out) return;  // (in place, and every value stays as it is)
+__device__ __forceinline__ void scale_part(const GradEntry& e, GradPart part, int tid, double coef, bool clean) {
+  if ((float)coef == 1.f && !clean && e.in == e.out) return;  // (in place, and every value stays as it is)
   if (e.in_type == F32) scale_part<THREADS, float>(e, part, tid, coef, clean);
   else if (e.in_type == BF16) scale_part<THREADS, __nv_bfloat16>(e, part, tid, coef, clean);
   else scale_part<THREADS, __half>(e, part, tid, coef, clean);
@@ -260,7 +267,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_grad_scale(const __grid_constant
     if (norm) *norm = (float)sqrt(stats.x);
     if (bad) *bad = (long long)stats.y;
   }
-  const float coef = clip_coefficient(stats.x, max_norm, eps);
+  const double coef = clip_coefficient(stats.x, max_norm, eps);
   const bool clean = zero && stats.y > 0.0;
   int i = t.count - 1;
   // (the chunks that this block had in the first pass, back from the last one)
@@ -335,7 +342,7 @@ __global__ void __launch_bounds__(GN_SMALL_THREADS)
     if (bad) *bad = (long long)v.y;
   }
   if (!scale) return;
-  const float coef = clip_coefficient(v.x, max_norm, eps);
+  const double coef = clip_coefficient(v.x, max_norm, eps);
   const bool clean = zero && v.y > 0.0;
   for (int c = first; c < t.chunks; c += step) {
     const GradEntry& e = entry(c);
