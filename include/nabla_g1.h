@@ -203,8 +203,9 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
  * of non-finite values. zero_nonfinite: those count as 0 in S and are written as 0; otherwise they take part as the
  * arithmetic has them (S infinite or NaN).
  *   sumsq: stats (2 doubles, 16-byte aligned) = S, bad; ranks that share a model add theirs up before the next call.
- *   scale: c = min(1, max_norm / (sqrt(S) + eps)), outs[i] = c grads[i] in type out_types[i]; norm = sqrt(S) and bad,
- *     each where not NULL. An output may be its own gradient (same address and type); outputs that overlap anything
+ *   scale: c = 1 where sqrt(S) + eps <= max_norm (so always under an infinite bound, unless S is NaN), else max_norm /
+ *     (sqrt(S) + eps): 0 for an infinite S, NaN for a NaN one; outs[i] = c grads[i] in type out_types[i]; norm = sqrt(S)
+ *     and bad, each where not NULL (the norm is told in float32: infinite where it rounds to that). An output may be its own gradient (same address and type); outputs that overlap anything
  *     else are refused. outs NULL: norm and bad alone.
  *   clip: sumsq, then scale.
  * work: nb_g1_grad_work_bytes(count) bytes, 16-byte aligned; clip takes none (NULL) for a list of at most

@@ -1,5 +1,6 @@
 // The global norm of a list of tensors and the list times the clip coefficient:
-//   S = sum g^2 over every value of every tensor, norm = sqrt(S), c = min(1, max_norm / (norm + eps)), out = c g
+//   S = sum g^2 over every value of every tensor, norm = sqrt(S), out = c g,
+//   c = 1 where norm + eps <= max_norm, else max_norm / (norm + eps)
 // Non-finite values are counted; with `zero` they count as 0 in S and in out.
 //
 // S is held in 64 bits, so neither a gradient of 1e30 overflows it nor one of 1e-30 vanishes from it. Eight squares at

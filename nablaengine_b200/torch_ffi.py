@@ -704,12 +704,12 @@ def grad_norm(grads, *, nonfinite="keep", group=None):
 
 
 def clip_grad_norm(grads, max_norm, *, eps=CLIP_EPS, nonfinite="keep", out=None, group=None):
-    """Scale a list of gradients by min(1, max_norm / (norm + eps)), norm and bad as grad_norm's, which are returned.
-    In place, or into `out`: as many dense tensors, of the gradients' shapes and strides, each of its gradient's type or
-    float32. nonfinite "keep": an infinite norm scales by 0 and a NaN norm by NaN, as the arithmetic has it; "zero":
-    non-finite values become 0 and the others are clipped by the norm without them. grads: dense CUDA tensors
-    (float32, bfloat16, float16, mixed) on one device, no two overlapping. Under torch.no_grad semantics: nothing is
-    differentiated through."""
+    """Scale a list of gradients by max_norm / (norm + eps) unless norm + eps <= max_norm (an infinite bound leaves them
+    as they are), norm and bad as grad_norm's, which are returned. In place, or into `out`: as many dense tensors, of the
+    gradients' shapes and strides, each of its gradient's type or float32. nonfinite "keep": under a finite bound an
+    infinite norm scales by 0, and a NaN norm by NaN under any, as the arithmetic has it; "zero": non-finite values
+    become 0 and the others are clipped by the norm without them. grads: dense CUDA tensors (float32, bfloat16, float16,
+    mixed) on one device, no two overlapping. Under torch.no_grad semantics: nothing is differentiated through."""
     grads = _tensor_list("grads", grads)
     outs = grads if out is None else _tensor_list("out", out)
     return _clip_impl(grads, outs, max_norm, eps, _zero_mode(nonfinite), group)

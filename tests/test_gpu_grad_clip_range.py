@@ -54,3 +54,21 @@ def test_non_finite_values_zeroed_under_a_subnormal_coefficient():
     grads[4][-1] = float("-inf")
     _check(grads, 1e-3, zero=True)
     assert all(torch.isfinite(g).all() for g in grads)
+
+
+def test_an_infinite_bound():
+    """norm + eps <= infinity holds for an infinite norm too: nothing is scaled; a NaN norm scales by NaN."""
+    torch = _torch()
+    from nablaengine_b200 import torch_ffi
+    inf, nan = float("inf"), float("nan")
+    for scale in (1.0, 1e38):
+        g = [torch.tensor([1.0 * scale, -inf], device="cuda"), torch.tensor([3.0], device="cuda")]
+        norm, bad = torch_ffi.clip_grad_norm(g, inf)
+        assert float(norm) == inf and int(bad) == 1
+        assert torch.equal(g[0], torch.tensor([1.0 * scale, -inf], device="cuda")) and g[1].tolist() == [3.0]
+    g = [torch.tensor([1.0, nan, inf], device="cuda")]
+    norm, bad = torch_ffi.clip_grad_norm(g, inf)
+    assert torch.isnan(norm) and int(bad) == 2 and torch.isnan(g[0]).all()
+    g = [torch.tensor([1.0, nan, inf], device="cuda")]
+    torch_ffi.clip_grad_norm(g, inf, nonfinite="zero")
+    assert g[0].tolist() == [1.0, 0.0, 0.0]
