@@ -70,9 +70,8 @@ int gpu_of(const Tensor& t) { return t.get_device(); }
 
 void* at_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-void check(int rc, const char* entry, const char* refused = nullptr) {
+void check(int rc, const char* entry) {
   if (rc == 0) return;
-  if (rc == 1 && refused) refuse(PyExc_ValueError, refused);  // cudaErrorInvalidValue, before any launch
   refuse(PyExc_RuntimeError, std::string(entry) + " failed (CUDA error " + std::to_string(rc) + ")");
 }
 
@@ -242,8 +241,22 @@ List outs_of(PyObject* x, PyObject* grads, const List& g) {
   return o;
 }
 
-constexpr const char* OVERLAP =
-    "a clipped gradient may not share memory with another gradient or output (but may be its own gradient)";
+// The result of a clip's entry: it refuses outputs that share memory, which is told as such; anything else is an error.
+void check_clip(int rc, const char* entry, const List& g, const List* o) {
+  if (rc == 0) return;
+  const auto meet = [](const List& a, size_t i, const List& b, size_t k) {
+    const char *x = static_cast<const char*>(a.at[i]), *y = static_cast<const char*>(b.at[k]);
+    return x < y + b.t[k]->nbytes() && y < x + a.t[i]->nbytes();
+  };
+  for (size_t i = 0; o && i < g.t.size(); i++)
+    for (size_t k = 0; k < g.t.size(); k++) {
+      const bool own = i == k && g.at[i] == o->at[i] && g.types[i] == o->types[i];
+      if ((!own && meet(*o, i, g, k)) || (i != k && meet(*o, i, *o, k)))
+        refuse(PyExc_ValueError, "out[" + std::to_string(i) + "] and " + std::to_string(k) + ": a clipped gradient may "
+                                 "not share memory with another gradient or output (but may be its own gradient)");
+    }
+  check(rc, entry);
+}
 
 Tensor empty_on(int device, at::IntArrayRef sizes, at::ScalarType type) {
   return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
@@ -285,14 +298,14 @@ std::vector<Tensor> grad_clip(PyObject* const* a) {
     for (long long n : g.sizes) values += n;
     Tensor work;
     if (count > NB_G1_GRAD_SMALL_TENSORS || values > NB_G1_GRAD_SMALL_VALUES) work = work_for(g);
-    check(nb_g1_grad_clip(stream, count, g.at.data(), outs, g.sizes.data(), g.types.data(), o.types.data(), zero,
-                          max_norm, eps, at_or_null(work), norm.data_ptr<float>(), badp),
-          "nb_g1_grad_clip", OVERLAP);
+    check_clip(nb_g1_grad_clip(stream, count, g.at.data(), outs, g.sizes.data(), g.types.data(), o.types.data(), zero,
+                               max_norm, eps, at_or_null(work), norm.data_ptr<float>(), badp),
+               "nb_g1_grad_clip", g, outs ? &o : nullptr);
   } else {
     const Tensor& stats = THPVariable_Unpack(a[5]);
-    check(nb_g1_grad_scale(stream, count, g.at.data(), outs, g.sizes.data(), g.types.data(), o.types.data(), zero,
-                           max_norm, eps, stats.data_ptr<double>(), norm.data_ptr<float>(), badp),
-          "nb_g1_grad_scale", OVERLAP);
+    check_clip(nb_g1_grad_scale(stream, count, g.at.data(), outs, g.sizes.data(), g.types.data(), o.types.data(), zero,
+                                max_norm, eps, stats.data_ptr<double>(), norm.data_ptr<float>(), badp),
+               "nb_g1_grad_scale", g, outs ? &o : nullptr);
   }
   if (outs)
     for (const Tensor* t : o.t)
