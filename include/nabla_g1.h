@@ -181,7 +181,8 @@ int nb_g1_diag_forward_ex(cudaStream_t stream, unsigned long long* counters, int
  * 2 float16. As every entry: asynchronous on `stream`, the caller owns every buffer, arguments out of range return
  * cudaErrorInvalidValue before anything is launched, and results repeat bit for bit (no atomics).
  *
- * Layer norm of x (rows, cols), rows `stride` values apart (0: every row the same), y and g_x dense:
+ * Layer norm of x (rows, cols), rows `stride` values apart (0: every row the same; rows times cols or stride: at most
+ * 2^40), y and g_x dense; no output may overlap an input or another output:
  *   mean = sum x / cols, rstd = (sum (x - mean)^2 / cols + eps)^(-1/2), y = (x - mean) rstd weight + bias
  * weight and bias (cols,) of type wtype, which is float32 or x's; each may be NULL (1 and 0). mean, rstd (rows,).
  * The backward takes g_y (rows `g_stride` apart, x's type) and the forward's mean and rstd:

@@ -16,22 +16,25 @@ using namespace nbtrain;
 namespace {
 
 // ---- arguments ------------------------------------------------------------------------------------------------------
-bool ln_args_ok(long long rows, long long cols, long long stride, int dtype, int wtype) {
-  return rows >= 0 && cols >= 1 && cols <= INT_MAX / 4 && stride >= 0 && dtype_ok(dtype) &&
-         (wtype == F32 || wtype == dtype);
+constexpr long long LONGEST = 1ll << 40;  // values of a tensor: more than any GPU holds
+
+bool ln_size_ok(long long rows, long long cols) {
+  return rows >= 0 && cols >= 1 && cols <= INT_MAX / 4 && rows <= LONGEST / cols;
 }
+bool ln_stride_ok(long long rows, long long stride) {
+  return stride >= 0 && stride <= LONGEST / std::max(rows, 1ll);
+}
+bool ln_types_ok(int dtype, int wtype) { return dtype_ok(dtype) && (wtype == F32 || wtype == dtype); }
 
 bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) == 0; }
 
 // ---- the gradient list ----------------------------------------------------------------------------------------------
-constexpr long long GRAD_LONGEST = 1ll << 40;  // values of a tensor: more than any GPU holds
-
 bool grads_ok(int count, const void* const* in, const long long* sizes, const int* types) {
   if (count < 0) return false;
   if (count == 0) return true;
   if (!in || !sizes || !types) return false;
   for (int i = 0; i < count; i++)
-    if (sizes[i] < 0 || sizes[i] > GRAD_LONGEST || !dtype_ok(types[i]) ||
+    if (sizes[i] < 0 || sizes[i] > LONGEST || !dtype_ok(types[i]) ||
         (sizes[i] && (!in[i] || !aligned(in[i], types[i]))))
       return false;
   return true;
@@ -207,14 +210,15 @@ bool results_ok(const float* norm, const long long* bad) {
 extern "C" {
 
 long long nb_g1_layer_norm_work_bytes(long long rows, long long cols) {
-  if (rows < 0 || cols < 1 || cols > INT_MAX / 4) return -1;
+  if (!ln_size_ok(rows, cols)) return -1;
   return ln_max_parts(rows, (int)cols) * 2 * cols * 4;
 }
 
 int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols, long long stride, int dtype,
                              const void* x, int wtype, const void* weight, const void* bias, float eps, void* y,
                              float* mean, float* rstd) {
-  if (!ln_args_ok(rows, cols, stride, dtype, wtype) || !(eps >= 0.f) || !std::isfinite(eps))
+  if (!ln_size_ok(rows, cols) || !ln_stride_ok(rows, stride) || !ln_types_ok(dtype, wtype) || !(eps >= 0.f) ||
+      !std::isfinite(eps))
     return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   if (!x || !y || !mean || !rstd || !aligned(x, dtype) || !aligned(y, dtype) || !aligned(weight, wtype) ||
@@ -228,7 +232,9 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
                               long long stride, int dtype, const void* g_y, const void* x, const float* mean,
                               const float* rstd, int wtype, const void* weight, void* g_x, void* g_weight,
                               void* g_bias, void* work) {
-  if (!ln_args_ok(rows, cols, stride, dtype, wtype) || g_stride < 0) return (int)cudaErrorInvalidValue;
+  if (!ln_size_ok(rows, cols) || !ln_stride_ok(rows, stride) || !ln_stride_ok(rows, g_stride) ||
+      !ln_types_ok(dtype, wtype))
+    return (int)cudaErrorInvalidValue;
   if ((rows && (!g_y || !x || !mean || !rstd)) || !aligned(g_y, dtype) || !aligned(x, dtype) ||
       !aligned(g_x, dtype) || !aligned(weight, wtype) || !aligned(g_weight, wtype) || !aligned(g_bias, wtype) ||
       !aligned(mean, F32) || !aligned(rstd, F32))
