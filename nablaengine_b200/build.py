@@ -18,7 +18,11 @@ LIBDIR = PKG / "lib"
 LIB = LIBDIR / "libnabla_g1.so"
 SOURCES = [CSRC / n for n in ("nb_g1.cu", "nb_train.cu", "nb_layer_norm_f32.cu", "nb_layer_norm_bf16.cu",
                               "nb_layer_norm_f16.cu")]
-DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [PKG.parent / "include" / "nabla_g1.h"]
+# What the library exports: its C entries alone. Its kernels' host functions and what it remembers per kernel and device
+# would otherwise be shared with another copy in the process (the profile build's, or a program's that compiles them in).
+EXPORTS = CSRC / "nabla_g1.map"
+DEPS = (SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+        + [EXPORTS, PKG.parent / "include" / "nabla_g1.h"])
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared", "--cudart", "shared"]
 
@@ -98,7 +102,8 @@ def build(force=False, verbose=False, extra=(), out=None):
         return lib
     LIBDIR.mkdir(exist_ok=True)
     tmp = lib.with_suffix(f".tmp{os.getpid()}.so")
-    cmd = [nvcc(), *ARCH, *FLAGS, *extra, "--threads", "0", "-o", str(tmp), *map(str, SOURCES)]
+    cmd = [nvcc(), *ARCH, *FLAGS, *extra, "-Xlinker", f"--version-script={EXPORTS}", "--threads", "0", "-o", str(tmp),
+           *map(str, SOURCES)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), flush=True)
