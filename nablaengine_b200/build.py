@@ -5,6 +5,7 @@ nvcc cross-compiles without a GPU, so this runs anywhere the CUDA toolkit is ins
 the repository to the GPU machines. `python -m nablaengine_b200.build` rebuilds when a source is newer than the
 library or the library was built with other nvcc flags (recorded in a stamp file beside it).
 """
+import hashlib
 import os
 import shutil
 import subprocess
@@ -58,6 +59,21 @@ TORCH_LIB = LIBDIR / "nb_torch.so"
 TORCH_DEPS = [CSRC / "nb_torch.cpp", PKG.parent / "include" / "nabla_g1.h"]
 
 
+def _torch_key():
+    """What nb_torch.so was built from and for: torch (whose inline C++ types it holds), Python and the sources. No path:
+    a built tree may be moved."""
+    import torch
+    sources = hashlib.sha256(b"".join(p.read_bytes() for p in TORCH_DEPS)).hexdigest()
+    return (f"torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} "
+            f"python {sysconfig.get_config_var('SOABI')} sources {sources}")
+
+
+def torch_stale():
+    """True when nb_torch.so is missing, or was built from other sources or for another torch or Python."""
+    stamp = _stamp(TORCH_LIB)
+    return not TORCH_LIB.exists() or not stamp.exists() or stamp.read_text() != _torch_key()
+
+
 def _torch_command(out):
     """The host compiler's command for nb_torch.so (torch's and Python's headers, libnabla_g1.so beside it)."""
     import torch
@@ -69,24 +85,21 @@ def _torch_command(out):
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include],
             str(TORCH_DEPS[0]), "-o", str(out), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
             "-ltorch_cuda", "-ltorch_python", f"-L{LIBDIR}", "-lnabla_g1", "-Wl,-rpath,$ORIGIN",
-            f"-Wl,-rpath,{root / 'lib'}"], torch.__version__
+            f"-Wl,-rpath,{root / 'lib'}"]
 
 
 def build_torch(force=False):
-    """Compile nb_torch.so (the host side of the training operators) when it is missing, older than its sources or
-    built for another torch; returns its path. libnabla_g1.so has to be there."""
-    tmp = TORCH_LIB.with_suffix(f".tmp{os.getpid()}.so")
-    cmd, version = _torch_command(tmp)
-    text = " ".join([version, *cmd[:-1]]).replace(str(tmp), "")
-    stamp = _stamp(TORCH_LIB)
-    if (not force and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == text
-            and all(p.stat().st_mtime <= TORCH_LIB.stat().st_mtime for p in TORCH_DEPS)):
+    """Compile nb_torch.so (the host side of the training operators) when it is stale; returns its path. libnabla_g1.so
+    has to be there."""
+    if not force and not torch_stale():
         return TORCH_LIB
+    tmp = TORCH_LIB.with_suffix(f".tmp{os.getpid()}.so")
+    cmd = _torch_command(tmp)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
         raise RuntimeError(f"{cmd[0]} failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, TORCH_LIB)
-    stamp.write_text(text)
+    _stamp(TORCH_LIB).write_text(_torch_key())
     return TORCH_LIB
 
 

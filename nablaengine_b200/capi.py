@@ -99,15 +99,16 @@ def load(path=None, build_if_missing=True):
 
 def load_torch(build_if_missing=True):
     """The loaded torch host module nb_torch (the training operators' checks, outputs and calls); builds it first when
-    it is missing and a compiler exists."""
+    it is missing, or was built from other sources or for another torch, and a compiler exists."""
     load(build_if_missing=build_if_missing)  # (nb_torch is linked against it)
     with _LOCK:
         if not _TORCH:
             import importlib.util
             import torch  # noqa: F401  (its libraries have to be there)
-            if not _build.TORCH_LIB.exists():
+            if _build.torch_stale():
                 if not build_if_missing:
-                    raise RuntimeError(f"{_build.TORCH_LIB} is missing: run `python -m nablaengine_b200.build`")
+                    raise RuntimeError(f"{_build.TORCH_LIB} is missing, or was built from other sources or for another "
+                                       "torch: run `python -m nablaengine_b200.build`")
                 _build.build_torch()
             spec = importlib.util.spec_from_file_location("nb_torch", _build.TORCH_LIB)
             module = importlib.util.module_from_spec(spec)
