@@ -215,9 +215,11 @@ def _device(index):
 
 def init(device=None):
     """Load the library and prepare `device` (default: torch's current CUDA device); idempotent per device. The
-    first call on a device synchronises it once: make it before capturing a CUDA graph. It also makes the autograd
-    functions and custom ops, which torch.compile cannot make while it traces."""
+    first call on a device synchronises it once: make it before capturing a CUDA graph. It also loads the training
+    operators' host module and makes the autograd functions and custom ops, which torch.compile cannot make while it
+    traces."""
     _device(_device_index(device))
+    _prepare_native()
     _autograd_function("step")
     custom_ops()
     return {"library": str(capi._build.LIB), "nq": NQ, "nv": NV, "nu": NU, "nbody": NBODY, "maxcon": MAXCON}
@@ -353,6 +355,15 @@ def _native():
     if not _NATIVE:
         _NATIVE.append(capi.load_torch())
     return _NATIVE[0]
+
+
+def _prepare_native():
+    """Load the compiled host module ahead of its first call. The step does not need it: where it cannot be loaded or
+    built, the first call of an operator that does says why."""
+    try:
+        _native()
+    except (RuntimeError, ImportError, OSError):
+        pass
 
 
 def _tensor_list(name, x):

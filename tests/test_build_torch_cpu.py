@@ -63,3 +63,19 @@ def test_any_other_module_is_built_again_or_refused(module, monkeypatch, change)
     with pytest.raises(_Rebuilt):
         capi.load_torch()
     assert not capi._TORCH
+
+
+def test_preparing_a_device_does_not_need_the_module(monkeypatch):
+    """Where the module cannot be loaded, only the calls that need it say so."""
+    import torch
+    from nablaengine_b200 import torch_ffi
+
+    for kind in (RuntimeError, ImportError, FileNotFoundError):
+        def fails(build_if_missing=True):
+            raise kind("cannot be built here")
+
+        monkeypatch.setattr(torch_ffi, "_NATIVE", [])
+        monkeypatch.setattr(capi, "load_torch", fails)
+        torch_ffi._prepare_native()
+        with pytest.raises(kind, match="cannot be built here"):
+            torch_ffi.layer_norm(torch.zeros(2, 3))
