@@ -2,8 +2,8 @@
 // from torch's allocator, and the calls of libnabla_g1's C entries on torch's current stream. It is compiled because a
 // call's time on the host is what a small layer or a list of many small gradients costs.
 //
-// Every function raises TypeError for a tensor it cannot take and ValueError for an option out of range, before any
-// launch; nothing is cast or copied.
+// Every function raises TypeError for a tensor it cannot take, NotImplementedError for one with a forward-mode tangent
+// and ValueError for an option out of range, before any launch; nothing is cast or copied.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -58,10 +58,12 @@ int code_of(const Tensor& t) {
 }
 
 // A tensor argument: its tensor if it is one on a GPU of a value type whose memory holds its values (no lazy negation),
-// else null.
+// else null. One that carries a forward-mode tangent is refused: the calls here read memory past the dispatcher and
+// would drop it.
 const Tensor* gpu_tensor(PyObject* x) {
   if (!THPVariable_Check(x)) return nullptr;
   const Tensor& t = THPVariable_Unpack(x);
+  if (t._fw_grad(0).defined()) refuse(PyExc_NotImplementedError, "forward-mode derivatives are not available");
   const bool plain = t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !t._is_zerotensor();
   return plain && code_of(t) >= 0 ? &t : nullptr;
 }

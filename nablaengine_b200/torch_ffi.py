@@ -583,6 +583,17 @@ def _tracing():
     return torch.compiler.is_compiling()
 
 
+def _refuse_tangents(*xs):
+    """The step's kernels compute no forward-mode derivatives: a tensor that has a tangent is refused, not stripped of
+    it. (The training operators' host module refuses its own.)"""
+    import torch
+    forward_ad = torch.autograd.forward_ad
+    if forward_ad._current_level >= 0:  # (inside a dual_level; nothing else is asked outside of one)
+        for x in xs:
+            if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+                raise _fail("forward-mode derivatives are not available", NotImplementedError)
+
+
 def _differentiating(*xs):
     import torch
     return torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in xs)
@@ -634,6 +645,7 @@ def kinematics(qpos, qvel, com):
     """The kinematics outputs of states (qpos, qvel, com) (reference torch_ffi.py:838; semantics
     g1_engine/kinematics.py:1-47): (qpos_n (B, 36), xpos (B, 31, 3), xquat (B, 31, 4), cvel (B, 31, 6),
     subtree_com (B, 31, 3)), differentiable in qpos and qvel (com gets no gradient)."""
+    _refuse_tangents(qpos, qvel, com)
     if _differentiating(qpos, qvel, com):
         return _autograd_function("kinematics").apply(qpos, qvel, com)
     return tuple(custom_ops()["kinematics"](qpos, qvel, com))
@@ -654,6 +666,7 @@ def step(qpos, qvel, warm, ctrl, friction, com, *, iterations=ITERATIONS, subste
     if not math.isfinite(opts["grad_decay"]):
         raise _fail(f"grad_decay must be finite, got {grad_decay}", ValueError)
     state = (qpos, qvel, warm, ctrl, friction, com)
+    _refuse_tangents(*state)
     if _differentiating(*state):
         q1, v1, w1 = _autograd_function("step").apply(*state, opts)
     else:
@@ -682,7 +695,7 @@ def layer_norm(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
     """Layer norm over x's last dimension: (x - mean) * rstd [* weight] [+ bias], with the row's mean and rstd =
     1 / sqrt(variance + eps), in x's type and shape (dense). x: (..., columns), float32, bfloat16 or float16, rows one
     stride apart (a column slice of a wider buffer is read in place); weight, bias: (columns,), both float32 or both
-    x's type. The arithmetic is float32, rounded once. Differentiable (once) in x, weight and bias."""
+    x's type. The arithmetic is float32, rounded once. Differentiable (once, in reverse mode) in x, weight and bias."""
     if _differentiating(x, weight, bias):
         return _autograd_function("layer_norm").apply(x, weight, bias, float(eps))
     return layer_norm_forward(x, weight, bias, eps)[0]
@@ -716,8 +729,8 @@ def grad_norm(grads, *, nonfinite="keep", group=None):
 
 def clip_grad_norm(grads, max_norm, *, eps=CLIP_EPS, nonfinite="keep", out=None, group=None):
     """Scale a list of gradients by max_norm / (norm + eps) unless norm + eps <= max_norm (an infinite bound leaves them
-    as they are), norm and bad as grad_norm's, which are returned. In place, or into `out`: as many dense tensors, of the
-    gradients' shapes and strides, each of its gradient's type or float32. nonfinite "keep": under a finite bound an
+    as they are), norm and bad as grad_norm's, which are returned. In place, or into `out`: as many dense tensors, of
+    the gradients' shapes and strides, each of its gradient's type or float32. nonfinite "keep": under a finite bound an
     infinite norm scales by 0, and a NaN norm by NaN under any, as the arithmetic has it; "zero": non-finite values
     become 0 and the others are clipped by the norm without them. grads: dense CUDA tensors (float32, bfloat16, float16,
     mixed) on one device, no two overlapping. Under torch.no_grad semantics: nothing is differentiated through."""
