@@ -697,6 +697,7 @@ def layer_norm(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
     stride apart (a column slice of a wider buffer is read in place); weight, bias: (columns,), both float32 or both
     x's type. The arithmetic is float32, rounded once. Differentiable (once, in reverse mode) in x, weight and bias."""
     if _differentiating(x, weight, bias):
+        _refuse_tangents(x, weight, bias)
         return _autograd_function("layer_norm").apply(x, weight, bias, float(eps))
     return layer_norm_forward(x, weight, bias, eps)[0]
 
