@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -268,8 +269,18 @@ Tensor work_for(const List& g) {
   return empty_on(g.device, {(int64_t)nb_g1_grad_work_bytes((int)g.t.size())}, at::kByte);
 }
 
+// The two calls below write in place and have no operation that a trace could hold: it would hold their results.
+void refuse_trace() {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
+      TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE))
+    refuse(PyExc_NotImplementedError, "grad_norm and clip_grad_norm cannot be traced");
+}
+
 // (grads, zero) -> stats (2,) float64: the sum of squares and the number of non-finite values
 std::vector<Tensor> grad_sumsq(PyObject* const* a) {
+  refuse_trace();
   const List g = list_of("grads", a[0]);
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)g.device);
   const Tensor work = work_for(g), stats = empty_on(g.device, {2}, at::kDouble);
@@ -281,6 +292,7 @@ std::vector<Tensor> grad_sumsq(PyObject* const* a) {
 
 // (grads, outs or None, max_norm, eps, zero, stats or None) -> (norm, bad): by grads' own sums, or by stats'
 std::vector<Tensor> grad_clip(PyObject* const* a) {
+  refuse_trace();
   const List g = list_of("grads", a[0]);
   const double max_norm = number(a[2]), eps = number(a[3]);
   if (!(max_norm >= 0) || !(eps >= 0) || !std::isfinite(eps))

@@ -577,10 +577,11 @@ def _autograd_function(name):
 
 
 def _tracing():
-    """True while torch.compile traces: the library calls then go through their custom ops (opaque graph nodes);
-    eager calls go straight to the implementation (the same launches, without the dispatcher's overhead)."""
+    """True while torch.compile traces or a torch dispatch mode (make_fx's, a FakeTensorMode, ...) is active: the
+    library calls then go through their custom ops (opaque graph nodes); eager calls go straight to the implementation
+    (the same launches, without the dispatcher's overhead)."""
     import torch
-    return torch.compiler.is_compiling()
+    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
 
 
 def _refuse_tangents(*xs):
