@@ -1,8 +1,9 @@
 """A control policy trained through the differentiable control step: a small network reads each world's state (qpos,
 qvel and the last ctrl), sets the PD setpoints of the next step, and learns from the gradient of a T-step rollout's loss.
 It runs the training operators together as a learner uses them: the observation and every hidden layer are normalised by
-torch_ffi.layer_norm, the rollout goes through torch_ffi.step, and the gradients, which contacts can make very large or
-non-finite, are clipped by their global norm with torch_ffi.clip_grad_norm before the optimiser's step.
+torch_ffi.layer_norm, the rollout goes through torch_ffi.step, and the gradients, which contacts can make very large,
+are clipped by their global norm with torch_ffi.clip_grad_norm before the optimiser's step. A world that diverges, in
+its state or in its gradient, is left out before it enters the parameters' gradients, which are sums over the worlds.
 
   python -m nablaengine_b200.policy [--worlds 4096] [--steps 8] [--iterations 10] [--hidden 256,128]
 """
@@ -14,10 +15,16 @@ NQ, NV, NU = 36, 35, 29
 OBS = NQ + NV + NU
 
 
+def _finite_rows(x):
+    """(B, 1): the rows whose values are all finite (their sum is; one that overflows counts as lost too)."""
+    return x.sum(dim=1, keepdim=True) * 0 == 0
+
+
 def make_policy(hidden=(256, 128), seed=0, device="cpu", layer_norm=None):
     """A torch module: (qpos, qvel, last ctrl) -> setpoints' change. Normalised observation, then per hidden width a
     linear layer, a layer norm and an ELU, then a linear layer to the controls (small at the start, so that the first
-    rollouts stand). layer_norm: the operator (default torch_ffi.layer_norm; tests on CPU pass their own)."""
+    rollouts stand). A state that is not finite is seen as zeros: times its gradient, zero too, it would make the
+    weights' gradients NaN. layer_norm: the operator (default torch_ffi.layer_norm; tests on CPU pass their own)."""
     import torch
     if layer_norm is None:
         from .torch_ffi import layer_norm
@@ -45,22 +52,37 @@ def make_policy(hidden=(256, 128), seed=0, device="cpu", layer_norm=None):
             self.layers = torch.nn.Sequential(*layers)
 
         def forward(self, qpos, qvel, ctrl):
-            return self.layers(torch.cat([qpos, qvel, ctrl], dim=1))
+            x = torch.cat([qpos, qvel, ctrl], dim=1)
+            return self.layers(torch.where(_finite_rows(x), x, 0.0))
 
     with torch.random.fork_rng(devices=[]):
         torch.manual_seed(seed)
         return Policy().to(device)
 
 
-def rollout_loss(policy, inputs, steps, step_fn=None, scale=0.2, **step_kw):
+def rollout_loss(policy, inputs, steps, step_fn=None, scale=0.2, kept=None, **step_kw):
     """The mean over steps and worlds of |qvel|^2 of `steps` closed-loop control steps from the inputs' states (qpos,
-    qvel, warm, ctrl, friction, com): ctrl_t = the inputs' ctrl + scale * policy(state, ctrl_(t-1))."""
+    qvel, warm, ctrl, friction, com): ctrl_t = the inputs' ctrl + scale * policy(state, ctrl_(t-1)). The loss of a world
+    that diverges is not finite, and so is the mean; but where a step's gradient of a world's controls is not finite,
+    the backward takes zeros for it, so the parameters' gradient is that of the other worlds. kept: a list that the
+    backward appends the worlds (B, 1) to whose controls' gradient was finite, one tensor a step."""
+    import torch
     if step_fn is None:
         from .torch_ffi import step as step_fn
+
+    def finite_worlds(g):
+        finite = _finite_rows(g)
+        if kept is not None:
+            kept.append(finite)
+        return torch.where(finite, g, 0.0)
+
     q, v, w, base = (inputs[k] for k in ("qpos", "qvel", "warm", "ctrl"))
     ctrl, loss = base, 0.0
     for _ in range(steps):
-        ctrl = base + scale * policy(q, v, ctrl)
+        change = policy(q, v, ctrl)
+        if change.requires_grad:
+            change.register_hook(finite_worlds)
+        ctrl = base + scale * change
         q, v, w = step_fn(q, v, w, ctrl, inputs["friction"], inputs["com"], **step_kw)
         loss = loss + (v * v).sum() / (steps * v.shape[0])
     return loss
@@ -68,16 +90,19 @@ def rollout_loss(policy, inputs, steps, step_fn=None, scale=0.2, **step_kw):
 
 def train_step(policy, optimizer, inputs, steps, max_norm=1.0, clip=None, **rollout_kw):
     """One update: the rollout's loss, its gradient, the clip and the optimiser's step. Returns (loss, norm, bad): 0-d
-    tensors, the gradient's global norm before the clip and its non-finite values, which are zeroed. clip: the operator
+    tensors, the gradient's global norm before the clip, and what was not finite and is left out: the worlds' steps
+    whose controls' gradient was not, and any values of the parameters' gradients themselves. clip: the operator
     (default torch_ffi.clip_grad_norm)."""
+    import torch
     if clip is None:
         from .torch_ffi import clip_grad_norm as clip
     optimizer.zero_grad(set_to_none=True)
-    loss = rollout_loss(policy, inputs, steps, **rollout_kw)
+    kept = []
+    loss = rollout_loss(policy, inputs, steps, kept=kept, **rollout_kw)
     loss.backward()
     norm, bad = clip([p.grad for p in policy.parameters()], max_norm, nonfinite="zero")
     optimizer.step()
-    return loss.detach(), norm, bad
+    return loss.detach(), norm, bad + (~torch.cat(kept)).sum() if kept else bad
 
 
 def inputs_for(worlds, device="cpu"):
