@@ -100,7 +100,7 @@ def train_step(policy, optimizer, inputs, steps, max_norm=1.0, clip=None, **roll
     kept = []
     loss = rollout_loss(policy, inputs, steps, kept=kept, **rollout_kw)
     loss.backward()
-    norm, bad = clip([p.grad for p in policy.parameters()], max_norm, nonfinite="zero")
+    norm, bad = clip([p.grad for p in policy.parameters() if p.grad is not None], max_norm, nonfinite="zero")
     optimizer.step()
     return loss.detach(), norm, bad + (~torch.cat(kept)).sum() if kept else bad
 

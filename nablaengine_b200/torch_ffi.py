@@ -735,7 +735,8 @@ def clip_grad_norm(grads, max_norm, *, eps=CLIP_EPS, nonfinite="keep", out=None,
     the gradients' shapes and strides, each of its gradient's type or float32. nonfinite "keep": under a finite bound an
     infinite norm scales by 0, and a NaN norm by NaN under any, as the arithmetic has it; "zero": non-finite values
     become 0 and the others are clipped by the norm without them. grads: dense CUDA tensors (float32, bfloat16, float16,
-    mixed) on one device, no two overlapping. Under torch.no_grad semantics: nothing is differentiated through."""
+    mixed) on one device, no two overlapping (a parameter without a gradient, None, is the caller's to leave out). Under
+    torch.no_grad semantics: nothing is differentiated through."""
     grads = _tensor_list("grads", grads)
     outs = grads if out is None else _tensor_list("out", out)
     return _clip_impl(grads, outs, max_norm, eps, _zero_mode(nonfinite), group)
