@@ -368,6 +368,12 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), false), ln_per_sm
   if (SPLIT) cluster_barrier();  // (nobody leaves while others put sums into its slots)
 }
 
+// The sum of N terms (a power of two) in a tree, so that none passes through more than log2 N additions.
+template <int N, class F> __device__ __forceinline__ float tree_sum(F term) {
+  if constexpr (N == 1) return term(0);
+  else return tree_sum<N / 2>(term) + tree_sum<N / 2>([&](int k) { return term(k + N / 2); });
+}
+
 // The backward: both sums of a row (h and h xh) meet in one exchange; (x - mean) rstd is taken as written, not as one
 // fused product, which would leave rounding where x is the mean. part (gridDim.x, 2, cols), if wanted: the block's
 // column sums of g xh and g, which k_ln_backward_sum adds up in a fixed order.
@@ -473,12 +479,8 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
   store_sums<LANES, EPT, V, FULL>(mine + cols, cols, lane, gb);
   if (GROUPS == 1) return;
   __syncthreads();
-  for (int c = threadIdx.x; c < 2 * cols; c += THREADS) {
-    float v = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < GROUPS; k++) v += reinterpret_cast<const float*>(ring)[k * 2 * cols + c];
-    sums[c] = v;
-  }
+  for (int c = threadIdx.x; c < 2 * cols; c += THREADS)
+    sums[c] = tree_sum<GROUPS>([&](int k) { return reinterpret_cast<const float*>(ring)[k * 2 * cols + c]; });
 }
 
 // The backward of rows that one block does not take: a row to each team of t.split blocks (a cluster) of LANES threads,
@@ -637,9 +639,7 @@ __global__ void __launch_bounds__(32 * WARPS) k_ln_backward_sum(int parts, int c
   for (int i = threadIdx.x; i < 32 * V; i += 32 * WARPS) {
     const int at = blockIdx.x * 32 * V + i;
     if (at >= 2 * cols) continue;
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS; k++) t += s[k][i];
+    const float t = tree_sum<WARPS>([&](int k) { return s[k][i]; });
     if (at < cols) {
       if (gw) gw[at] = from_f32<W>(t);
     } else if (gb) {
