@@ -29,6 +29,13 @@ using at::Tensor;
 
 constexpr const char* WHERE = "nablaengine_b200.torch_ffi: ";
 
+// Thrown by a call that a dispatch mode (a trace, say) has to see: it returns None, and torch_ffi calls its custom op.
+struct Dispatched {};
+
+void leave_to_dispatcher() {
+  if (c10::impl::dispatch_mode_enabled()) throw Dispatched{};
+}
+
 struct Refused {
   PyObject* kind;
   std::string text;
@@ -136,6 +143,7 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
 
 // (x, weight, bias, eps) -> (y, mean, rstd)
 std::vector<Tensor> layer_norm(PyObject* const* a) {
+  leave_to_dispatcher();
   const Rows r = rows_of("x", a[0]);
   const Tensor& x = *r.t;
   const Tensor w = param("weight", a[1], x), b = param("bias", a[2], x);
@@ -166,6 +174,7 @@ const Tensor& statistic(const char* name, PyObject* p, const Tensor& x) {
 
 // (g_y, x, mean, rstd, weight, bias, want_x, want_weight, want_bias) -> (g_x, g_weight, g_bias), None where not wanted
 std::vector<Tensor> layer_norm_backward(PyObject* const* a) {
+  leave_to_dispatcher();
   const Rows r = rows_of("x", a[1]), g = rows_of("g_y", a[0]);
   const Tensor& x = *r.t;
   if (g.t->sizes() != x.sizes() || g.t->scalar_type() != x.scalar_type() || gpu_of(*g.t) != gpu_of(x))
@@ -273,6 +282,7 @@ Tensor work_for(const List& g) {
 void refuse_trace() {
   using c10::impl::TorchDispatchModeKey;
   using c10::impl::TorchDispatchModeTLS;
+  if (!c10::impl::dispatch_mode_enabled()) return;
   if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) ||
       TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE))
     refuse(PyExc_NotImplementedError, "grad_norm and clip_grad_norm cannot be traced");
@@ -348,6 +358,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
       PyTuple_SET_ITEM(t, (Py_ssize_t)i, x);
     }
     return t;
+  } catch (const Dispatched&) {
+    return Py_NewRef(Py_None);
   } catch (const Refused& e) {
     PyErr_SetString(e.kind, e.text.c_str());
     return nullptr;

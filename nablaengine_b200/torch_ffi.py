@@ -706,19 +706,25 @@ def layer_norm(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
 def layer_norm_forward(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
     """layer_norm without autograd: (y, mean, rstd), the rows' statistics in float32 with x's leading dimensions, which
     layer_norm_backward takes."""
-    if _tracing():
-        return tuple(custom_ops()["layer_norm"](x, weight, bias, float(eps)))
-    return _native().layer_norm(x, weight, bias, eps)
+    import torch
+    if not torch.compiler.is_compiling():
+        r = _native().layer_norm(x, weight, bias, eps)
+        if r is not None:  # (None: a dispatch mode has to see the call)
+            return r
+    return tuple(custom_ops()["layer_norm"](x, weight, bias, float(eps)))
 
 
 def layer_norm_backward(g_y, x, mean, rstd, weight=None, bias=None):
     """The gradients of layer_norm_forward(x, weight, bias) from the cotangent g_y (x's type and shape): (g_x,
     g_weight, g_bias), the last two in their parameters' types, None for a parameter that is None. They are summed over
     the rows in float32, in a fixed order."""
-    if _tracing():
-        gx, gw, gb = custom_ops()["layer_norm_backward"](g_y, x, mean, rstd, weight, bias, True, True, True)
-        return gx, None if weight is None else gw, None if bias is None else gb
-    return _native().layer_norm_backward(g_y, x, mean, rstd, weight, bias, True, True, True)
+    import torch
+    if not torch.compiler.is_compiling():
+        r = _native().layer_norm_backward(g_y, x, mean, rstd, weight, bias, True, True, True)
+        if r is not None:
+            return r
+    gx, gw, gb = custom_ops()["layer_norm_backward"](g_y, x, mean, rstd, weight, bias, True, True, True)
+    return gx, None if weight is None else gw, None if bias is None else gb
 
 
 def grad_norm(grads, *, nonfinite="keep", group=None):
