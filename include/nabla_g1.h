@@ -189,7 +189,9 @@ int nb_g1_diag_forward_ex(cudaStream_t stream, unsigned long long* counters, int
  *   h = g_y weight, xh = (x - mean) rstd, g_x = rstd (h - mean(h) - xh mean(h xh)),
  *   g_weight = sum over rows of g_y xh, g_bias = sum over rows of g_y (both of type wtype)
  * g_x, g_weight and g_bias may each be NULL (not wanted); work: nb_g1_layer_norm_work_bytes(rows, cols) bytes,
- * 16-byte aligned, needed for g_weight or g_bias. With no rows g_weight and g_bias are zero. Sums are float32. */
+ * 16-byte aligned, needed for g_weight or g_bias. With no rows g_weight and g_bias are zero. Sums are float32: a row
+ * the sum of whose squared deviations is beyond that has rstd 0 and y = bias; one whose squares vanish, with eps 0, an
+ * infinite rstd. */
 long long nb_g1_layer_norm_work_bytes(long long rows, long long cols);
 int nb_g1_layer_norm_forward(cudaStream_t stream, long long rows, long long cols, long long stride, int dtype,
                              const void* x, int wtype, const void* weight, const void* bias, float eps, void* y,
@@ -205,9 +207,10 @@ int nb_g1_layer_norm_backward(cudaStream_t stream, long long rows, long long col
  * arithmetic has them (S infinite or NaN).
  *   sumsq: stats (2 doubles, 16-byte aligned) = S, bad; ranks that share a model add theirs up before the next call.
  *   scale: c = 1 where sqrt(S) + eps <= max_norm (so always under an infinite bound, unless S is NaN), else max_norm /
- *     (sqrt(S) + eps): 0 for an infinite S, NaN for a NaN one; outs[i] = c grads[i] in type out_types[i]; norm = sqrt(S)
- *     and bad, each where not NULL (the norm is told in float32: infinite where it rounds to that). An output may be its own gradient (same address and type); outputs that overlap anything
- *     else are refused. outs NULL: norm and bad alone.
+ *     (sqrt(S) + eps): 0 for an infinite S, NaN for a NaN one; outs[i] = c grads[i] in type out_types[i]; norm =
+ *     sqrt(S) and bad, each where not NULL (the norm is told in float32: infinite where it rounds to that). An output
+ *     may be its own gradient (same address and type); outputs that overlap anything else are refused. outs NULL: norm
+ *     and bad alone.
  *   clip: sumsq, then scale.
  * work: nb_g1_grad_work_bytes(count) bytes, 16-byte aligned; clip takes none (NULL) for a list of at most
  * NB_G1_GRAD_SMALL_TENSORS tensors and NB_G1_GRAD_SMALL_VALUES values in all. */

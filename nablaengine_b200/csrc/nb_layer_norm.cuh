@@ -1,7 +1,8 @@
 // Layer norm over the last dimension (N columns, M rows), forward and backward.
 //   mean = sum x / N, var = sum (x - mean)^2 / N, rstd = (var + eps)^(-1/2), xh = (x - mean) rstd, y = xh w + b
 //   h = g w, c1 = sum h / N, c2 = sum h xh / N, gx = rstd (h - c1 - xh c2), gw = sum_rows g xh, gb = sum_rows g
-// Sums are float32; the variance is taken from the deviations (a second pass over registers), not from sum x^2.
+// Sums are float32; the variance is taken from the deviations (a second pass over registers), not from sum x^2. (Where
+// the squares' sum is beyond float32 rstd is 0; where it vanishes and eps is 0, infinite.)
 //
 // A block takes tiles of rows in turn. The tiles come through a ring of up to four stages in shared memory, filled by
 // asynchronous copies, so loads are in flight while a tile is worked on, and a dense x is copied in 16-byte pieces
@@ -12,7 +13,7 @@
 //
 // Memory bounds both directions (8 and 14 operations a value). 131072 x 512: forward bfloat16 50 us, 5.4 TB/s; backward
 // float32 139 us, 5.8 TB/s with the sum of the column sums (a plain copy reaches 6.55). 16-bit rows of an odd width are
-// bound by their instructions (values one by one: 65536 x 1001 float16 forward 71 us, backward 113), and the backward
+// bound by their instructions (values one by one: 65536 x 1001 float16 forward 74 us, backward 116), and the backward
 // of rows of more than 4096 columns by one block an SM, whose 16 warps meet at each row (8192 x 8192 bfloat16: 83 us,
 // 4.8 TB/s).
 #pragma once
@@ -487,8 +488,9 @@ __global__ void __launch_bounds__(ln_threads(LANES, sizeof(T), true), ln_per_sm(
 // t.width columns to a block. The two sums of a row meet in the slots of all its blocks
 // under the cluster's barrier, which is split: between arriving with row k's sums and waiting for the others' a thread
 // finishes row k - 1, from shared memory again: nobody stands still for the exchange, for half as many instructions
-// again (8192 x 8192 bfloat16, which needs no cluster, took 103 us here when k_ln_backward took 94). part (teams, 2,
-// cols), if wanted.
+// again (8192 x 8192 bfloat16, which needs no cluster, took 103 us here when k_ln_backward took 94; 4096 x 16384
+// bfloat16: 113 us, 3.6 TB/s; 4096 x 12000 float32: 223 us, 2.6 TB/s: the exchange and the second load bound it). part
+// (teams, 2, cols), if wanted.
 template <class T, int LANES, int V, bool FULL>
 __global__ void __launch_bounds__(LANES, 512 / LANES)
     k_ln_backward_split(LnTiles t, int gkind, long long gstride, int kind, long long stride, const T* __restrict__ gy,

@@ -696,7 +696,8 @@ def layer_norm(x, weight=None, bias=None, eps=LAYER_NORM_EPS):
     """Layer norm over x's last dimension: (x - mean) * rstd [* weight] [+ bias], with the row's mean and rstd =
     1 / sqrt(variance + eps), in x's type and shape (dense). x: (..., columns), float32, bfloat16 or float16, rows one
     stride apart (a column slice of a wider buffer is read in place); weight, bias: (columns,), both float32 or both
-    x's type. The arithmetic is float32, rounded once. Differentiable (once, in reverse mode) in x, weight and bias."""
+    x's type. The arithmetic is float32, rounded once (where the squared deviations' sum is beyond float32, rstd is 0).
+    Differentiable (once, in reverse mode) in x, weight and bias."""
     if _differentiating(x, weight, bias):
         _refuse_tangents(x, weight, bias)
         return _autograd_function("layer_norm").apply(x, weight, bias, float(eps))

@@ -1,5 +1,5 @@
-"""Every value of layer norm's results (torch_ffi.layer_norm_forward and _backward) against the definition in 64 bits, by
-checks that a NaN fails: every kernel's widths, the parameters' forms, and rows between poisoned neighbours."""
+"""Every value of layer norm's results (torch_ffi.layer_norm_forward and _backward) against the definition in 64 bits,
+by checks that a NaN fails: every kernel's widths, the parameters' forms, and rows between poisoned neighbours."""
 import pytest
 
 import layer_norm_checks as checks
@@ -22,8 +22,8 @@ def _check(x, w, b, gy, eps=1e-5):
     checks.check_backward(gy, x, mean, rstd, w, b, *torch_ffi.layer_norm_backward(gy, x, mean, rstd, w, b))
 
 
-# widths of every spread of a row over lanes, odd ones among them: inside a warp, over several, split over a cluster, and
-# beyond what is held in registers; row counts that fill no block and that fill many
+# widths of every spread of a row over lanes, odd ones among them: inside a warp, over several, split over a cluster,
+# and beyond what is held in registers; row counts that fill no block and that fill many
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,cols", [
     (1, 1), (1, 2), (5, 7), (9, 32), (17, 35), (64, 64), (257, 71), (4096, 100), (31, 128), (130, 255), (61, 256),
@@ -98,3 +98,16 @@ def test_column_sums_take_every_row_once(rows, cols, dtype):
 def test_column_sums_take_every_row_beyond_32_bits(cols):
     """More than 2^31 values, and rows on either side of that offset."""
     _check_sums(2 ** 31 // cols + 1000, cols, "bf16")
+
+
+@pytest.mark.parametrize("cols", [100, 5000, 20001, 40000])
+def test_beyond_float32s_squares(cols):
+    """The stated limit of the float32 sums: where the squared deviations' sum is infinite, rstd is 0 and y the bias."""
+    torch = _torch()
+    from nablaengine_b200 import torch_ffi
+    x, w, b, _ = checks.inputs(4, cols, "f32")
+    x[1] *= 1e25
+    y, mean, rstd = torch_ffi.layer_norm_forward(x, w, b)
+    assert float(rstd[1]) == 0.0 and torch.equal(y[1], b) and torch.isfinite(mean).all()
+    rest = [0, 2, 3]
+    checks.check_forward(x[rest], w, b, 1e-5, y[rest], mean[rest], rstd[rest])
